@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-enum { B200_F16 = 0, B200_BF16 = 1 };
+enum { B200_F16 = 0, B200_BF16 = 1, B200_F32 = 2 }; /* F32: logits of b200_sample_tokens only */
 enum { B200_I32 = 0, B200_I64 = 1 };
 
 enum {
@@ -335,6 +335,124 @@ B200_API int b200_build_slot_mapping(const void* block_tables, int32_t table_dty
                             int32_t num_blocks, void* slots_out, int32_t slots_dtype,
                             int64_t total_tokens, int32_t* cu_seqlens_out, uint32_t* error_word,
                             void* stream);
+
+/* ------------------------------------------- per-head norm + rotary + append
+ * No counterpart in the reference: an addition of this library.
+ *
+ * Decoders with a norm on every query and key head: RMS norm of each head of q
+ * and k (weights [head_dim] of the cache dtype), rotary embedding of the first
+ * rotary_dim dimensions and the K/V append, in one launch:
+ *     n(x, w)[i] = x[i] * rsqrt(mean(x^2) + eps) * w[i]
+ *     query_out  = rope(n(query, q_weight)),  K[layer, slot] = rope(n(key, k_weight)),
+ *     V[layer, slot] = value
+ * All arithmetic in 32 bits, one rounding at the end.  cos/sin hold one row of
+ * rotary_dim entries per token.  Any strides; last dimensions contiguous.
+ * Negative slots are skipped (q is still written); a slot past the pool sets
+ * B200_DEVERR_BAD_SLOT.
+ */
+typedef struct {
+  int64_t num_tokens;
+  int32_t num_q_heads;
+  int32_t layer;
+  int32_t rotary_dim; /* even, <= head_dim */
+  float eps;
+  int64_t q_stride_token, q_stride_head; /* elements */
+  int64_t k_stride_token, k_stride_head;
+  int64_t v_stride_token, v_stride_head;
+  int64_t q_out_stride_token, q_out_stride_head;
+  int64_t cos_stride_token, sin_stride_token;
+  int32_t slots_dtype; /* B200_I32 / B200_I64 */
+} b200_qk_norm_args;
+
+B200_API int b200_qk_norm_rope_append(const b200_cache_desc* cache, const b200_qk_norm_args* args,
+                             const void* query, const void* key, const void* value,
+                             const void* q_weight, const void* k_weight, const void* cos,
+                             const void* sin, const void* slots, void* query_out,
+                             uint32_t* error_word, void* stream);
+
+/* ------------------------------------------------------------------- pages
+ * No counterpart in the reference: additions of this library.
+ *
+ * Copy pages: for every pair i, in every layer, the first tokens[i] tokens
+ * (tokens == NULL: all block_size) of page src[i] of K and of V to page dst[i].
+ * src, dst and tokens are int32 or int64 arrays of num_pairs entries.  A negative
+ * id skips the pair, an id past the pool skips it and sets B200_DEVERR_BAD_BLOCK.
+ * No page may be the destination of two pairs, or a destination and a source.
+ */
+B200_API int b200_copy_kv_pages(const b200_cache_desc* cache, const void* src, const void* dst,
+                       const void* tokens, int32_t index_dtype, int64_t num_pairs,
+                       uint32_t* error_word, void* stream);
+
+/* Rewrite block tables to new page ids: out[r, c] = page_map[tables[r, c]], page_map
+ * int32 [num_blocks].  Negative entries (unused columns) stay; an entry past the
+ * pool stays and sets B200_DEVERR_BAD_BLOCK.  out may be tables itself.
+ */
+B200_API int b200_remap_block_tables(const void* tables, int32_t table_dtype, int64_t table_stride,
+                            int64_t num_rows, int32_t table_width, const int32_t* page_map,
+                            int32_t num_blocks, void* out, int64_t out_stride,
+                            uint32_t* error_word, void* stream);
+
+/* ---------------------------------------------------------------- sampling
+ * Replaces, for a whole batch and without host work, the per-request torch
+ * sampling of the reference's runner (hf_benchmark.py:581-605).
+ *
+ *   w_i = exp((logits_i - max) / temperature), tokens in order of w (ties: lowest
+ *   index); kept: w_i >= min_p, then the first top_k, then the smallest prefix
+ *   whose mass reaches top_p of what is left; token = first index whose running
+ *   kept mass passes uniform * (kept mass), masses in units of 2^-31 of the
+ *   largest, so the result does not depend on any order of addition.
+ * temperature <= 0 (or NaN): the first largest logit; its logprobs are those of
+ * temperature 1.  top_k <= 0 or >= vocab, top_p >= 1 (or NaN) and min_p <= 0 (or
+ * NaN) are off; top_p <= 0 keeps one token.  NaN logits count as -inf; a row of
+ * nothing else gives token -1 and logprobs -inf.
+ * logprobs: of the token under temperature alone; sampling_logprobs: under the
+ * kept tokens.  Arrays (one entry per row) override the scalars of args; each may
+ * be NULL.  vocab <= 376832.
+ */
+typedef struct {
+  int64_t rows;
+  int64_t row_stride; /* elements; rows contiguous */
+  int32_t vocab;
+  int32_t dtype; /* B200_F16 / B200_BF16 / B200_F32 */
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} b200_sample_args;
+
+B200_API int b200_sample_tokens(const b200_sample_args* args, const void* logits, const float* uniforms,
+                       const float* temperature, const int32_t* top_k, const float* top_p,
+                       const float* min_p, int64_t* tokens, float* logprobs,
+                       float* sampling_logprobs, void* stream);
+
+/* ------------------------------------------------- 8-bit projections (e4m3)
+ * No counterpart in the reference: additions of this library.
+ *
+ * Quantise: one fp32 scale per block_rows x 128 values (block_rows 1 for
+ * activations, 128 for weights): scale = max |x| / 448, q = rn(x * (448 / max |x|));
+ * a block whose largest magnitude is below 2^-100 becomes zeros with scale 0.
+ * scales[row / block_rows, column / 128] at the given element strides.
+ */
+B200_API int b200_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_t x_stride, int32_t dtype,
+                      int32_t block_rows, void* q, int64_t q_stride, float* scales,
+                      int64_t scale_stride_row, int64_t scale_stride_block, void* stream);
+
+/* out[m, n] = sum_b x_scales[m, b] w_scales[n / 128, b] sum_{k in block b} x[m, k] w[n, k]
+ * (+ bias[n]), blocks of 128 columns, 32-bit sums, rounded once to the output type.
+ * x [m, k] and w [n, k] are e4m3 with rows on 16-byte boundaries (x_stride and
+ * w_stride multiples of 16); bias (NULL: none) and out have type dtype.
+ */
+typedef struct {
+  int64_t m, n, k;
+  int64_t x_stride, w_stride, out_stride; /* elements between rows */
+  int64_t x_scale_stride_row, x_scale_stride_block;
+  int64_t w_scale_stride_row, w_scale_stride_block;
+  int32_t dtype; /* B200_F16 / B200_BF16 */
+} b200_fp8_linear_args;
+
+B200_API int b200_fp8_linear(const b200_fp8_linear_args* args, const void* x, const float* x_scales,
+                    const void* w, const float* w_scales, const void* bias, void* out,
+                    uint32_t* error_word, void* stream);
 
 /* ------------------------------------------------------------- validation
  * Device-side form of the reference wrappers' validate_inputs checks

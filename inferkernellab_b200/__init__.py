@@ -10,6 +10,12 @@ operators plus host mirrors of its cache, scheduler and runtime:
   into the attention launch;
 * ``paged_prefill_attention`` / ``paged_prefill_attention_varlen`` -- ragged
   causal prefill over the paged cache;
+* ``qk_norm_rope_append`` -- per-head RMS norm of q and k, rotary and append;
+* ``sample_tokens`` -- temperature / min-p / top-k / top-p sampling of a batch;
+* ``copy_kv_pages`` / ``remap_block_tables`` -- pages copied in every layer (a
+  request that forks, a pool that is compacted), tables rewritten;
+* ``quantize_fp8`` / ``quantize_fp8_weight`` / ``fp8_linear`` -- 8-bit projections
+  with block scales;
 * ``build_slot_mapping`` -- device-built slots + ``cu_seqlens`` for a batch;
 * ``PagedKVCache``, ``BlockAllocator``, ``TokenBudgetScheduler``,
   ``InferenceRuntime`` -- the reference's host-side contract;
@@ -22,21 +28,26 @@ build it with ``python -m inferkernellab_b200.build``.
 """
 
 from .cache import BlockAllocator, CacheLayout, PagedKVCache
+from .fp8 import fp8_linear, quantize_fp8, quantize_fp8_weight
 from .ops import (
     add_rmsnorm,
     append_kv,
     b200_available,
     build_slot_mapping,
     check_device_errors,
+    copy_kv_pages,
     paged_decode_attention,
     paged_decode_attention_append,
     paged_prefill_attention,
     paged_prefill_attention_varlen,
+    qk_norm_rope_append,
+    remap_block_tables,
     rope_append_kv,
     silu_mul,
 )
 from .prefix_cache import PrefixCache
 from .runtime import InferenceRuntime, RuntimeStats
+from .sampling import sample_tokens
 from .scheduler import InferenceRequest, ScheduleBatch, TokenBudgetScheduler
 
 BACKEND_NAME = "b200_paged"
@@ -65,12 +76,19 @@ __all__ = [
     "b200_available",
     "build_slot_mapping",
     "check_device_errors",
+    "copy_kv_pages",
+    "fp8_linear",
     "paged_decode_attention",
     "paged_decode_attention_append",
     "paged_decode_attention_b200",
     "paged_prefill_attention",
     "paged_prefill_attention_b200",
     "paged_prefill_attention_varlen",
+    "qk_norm_rope_append",
+    "quantize_fp8",
+    "quantize_fp8_weight",
+    "remap_block_tables",
     "rope_append_kv",
+    "sample_tokens",
     "silu_mul",
 ]

@@ -16,7 +16,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libb200_paged_attn.so"
 
-B200_F16, B200_BF16 = 0, 1
+B200_F16, B200_BF16, B200_F32 = 0, 1, 2
 B200_I32, B200_I64 = 0, 1
 
 B200_OK = 0
@@ -50,6 +50,12 @@ EXPORTED_SYMBOLS = (
     "b200_paged_prefill",
     "b200_build_slot_mapping",
     "b200_validate_decode_metadata",
+    "b200_qk_norm_rope_append",
+    "b200_copy_kv_pages",
+    "b200_remap_block_tables",
+    "b200_sample_tokens",
+    "b200_quantize_fp8",
+    "b200_fp8_linear",
     "b200_read_error_word",
     "b200_last_error",
     "b200_version",
@@ -141,6 +147,56 @@ class RopeAppendArgs(ctypes.Structure):
     ]
 
 
+class QkNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("num_tokens", ctypes.c_int64),
+        ("num_q_heads", ctypes.c_int32),
+        ("layer", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v_stride_token", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("q_out_stride_token", ctypes.c_int64),
+        ("q_out_stride_head", ctypes.c_int64),
+        ("cos_stride_token", ctypes.c_int64),
+        ("sin_stride_token", ctypes.c_int64),
+        ("slots_dtype", ctypes.c_int32),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+    ]
+
+
+class Fp8LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("w_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("x_scale_stride_row", ctypes.c_int64),
+        ("x_scale_stride_block", ctypes.c_int64),
+        ("w_scale_stride_row", ctypes.c_int64),
+        ("w_scale_stride_block", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
@@ -175,6 +231,19 @@ _PROTOTYPES = {
                                                _i32, _vp, _i32, _i64, _vp, _vp, _vp]),
     "b200_validate_decode_metadata": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _i32, _i32, _i32,
                                                      _i32, _vp, _vp]),
+    "b200_qk_norm_rope_append": (ctypes.c_int, [ctypes.POINTER(CacheDesc),
+                                                ctypes.POINTER(QkNormArgs), _vp, _vp, _vp, _vp,
+                                                _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200_copy_kv_pages": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _vp, _vp, _i32, _i64,
+                                          _vp, _vp]),
+    "b200_remap_block_tables": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _i64,
+                                               _vp, _vp]),
+    "b200_sample_tokens": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp, _vp, _vp, _vp, _vp,
+                                          _vp, _vp, _vp, _vp, _vp]),
+    "b200_quantize_fp8": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _i64,
+                                         _i64, _vp]),
+    "b200_fp8_linear": (ctypes.c_int, [ctypes.POINTER(Fp8LinearArgs), _vp, _vp, _vp, _vp, _vp,
+                                       _vp, _vp, _vp]),
     "b200_read_error_word": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint32), _i32, _vp]),
     "b200_last_error": (ctypes.c_char_p, []),
     "b200_version": (ctypes.c_char_p, []),

@@ -9,11 +9,16 @@
 #include "../../include/b200_paged_attn.h"
 #include "append.h"
 #include "decode.h"
+#include "fp8_linear.h"
+#include "fp8_quant.h"
 #include "host_common.h"
 #include "layer_ops.h"
 #include "metadata.h"
+#include "pages.h"
 #include "prefill.h"
+#include "qk_norm.h"
 #include "rope_append.h"
+#include "sample.h"
 
 namespace b200 {
 const char* last_error_cstr();
@@ -177,6 +182,67 @@ int b200_validate_decode_metadata(const void* block_tables, int32_t table_dtype,
                                                  table_width, context_lens, lens_dtype, num_seqs,
                                                  block_size, num_blocks, flags_out,
                                                  as_stream(stream));
+  });
+}
+
+int b200_qk_norm_rope_append(const b200_cache_desc* cache, const b200_qk_norm_args* args,
+                             const void* query, const void* key, const void* value,
+                             const void* q_weight, const void* k_weight, const void* cos,
+                             const void* sin, const void* slots, void* query_out,
+                             uint32_t* error_word, void* stream) {
+  return guarded([&] {
+    return b200::launch_qk_norm_rope_append(cache, args, query, key, value, q_weight, k_weight,
+                                            cos, sin, slots, query_out, error_word,
+                                            as_stream(stream));
+  });
+}
+
+int b200_copy_kv_pages(const b200_cache_desc* cache, const void* src, const void* dst,
+                       const void* tokens, int32_t index_dtype, int64_t num_pairs,
+                       uint32_t* error_word, void* stream) {
+  return guarded([&] {
+    return b200::launch_copy_kv_pages(cache, src, dst, tokens, index_dtype, num_pairs, error_word,
+                                      as_stream(stream));
+  });
+}
+
+int b200_remap_block_tables(const void* tables, int32_t table_dtype, int64_t table_stride,
+                            int64_t num_rows, int32_t table_width, const int32_t* page_map,
+                            int32_t num_blocks, void* out, int64_t out_stride,
+                            uint32_t* error_word, void* stream) {
+  return guarded([&] {
+    return b200::launch_remap_block_tables(tables, table_dtype, table_stride, num_rows,
+                                           table_width, page_map, num_blocks, out, out_stride,
+                                           error_word, as_stream(stream));
+  });
+}
+
+int b200_sample_tokens(const b200_sample_args* args, const void* logits, const float* uniforms,
+                       const float* temperature, const int32_t* top_k, const float* top_p,
+                       const float* min_p, int64_t* tokens, float* logprobs,
+                       float* sampling_logprobs, void* stream) {
+  return guarded([&] {
+    return b200::launch_sample_tokens(args, logits, uniforms, temperature, top_k, top_p, min_p,
+                                      tokens, logprobs, sampling_logprobs, as_stream(stream));
+  });
+}
+
+int b200_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_t x_stride, int32_t dtype,
+                      int32_t block_rows, void* q, int64_t q_stride, float* scales,
+                      int64_t scale_stride_row, int64_t scale_stride_block, void* stream) {
+  return guarded([&] {
+    return b200::launch_quantize_fp8(x, rows, cols, x_stride, dtype, block_rows, q, q_stride,
+                                     scales, scale_stride_row, scale_stride_block,
+                                     as_stream(stream));
+  });
+}
+
+int b200_fp8_linear(const b200_fp8_linear_args* args, const void* x, const float* x_scales,
+                    const void* w, const float* w_scales, const void* bias, void* out,
+                    uint32_t* error_word, void* stream) {
+  return guarded([&] {
+    return b200::launch_fp8_linear(args, x, x_scales, w, w_scales, bias, out, error_word,
+                                   as_stream(stream));
   });
 }
 

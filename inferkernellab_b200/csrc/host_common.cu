@@ -39,7 +39,7 @@ struct MapKeyHash {
 };
 std::unordered_map<MapKey, CUtensorMap, MapKeyHash> g_maps;
 
-// Key of a general 16-bit tiled map (encode_tensor_map_16b).
+// Key of a general 128-byte swizzled map (encode_tensor_map_16b / _8b).
 struct GenKey {
   const void* base;
   int rank, dtype;
@@ -206,16 +206,17 @@ int encode_cache_tensor_map(const b200_cache_desc* c, const void* base,
   return B200_OK;
 }
 
-int encode_tensor_map_16b(const void* base, int rank, const uint64_t* dims,
-                          const uint64_t* strides_bytes, const uint32_t* box, int dtype,
-                          CUtensorMap* out) {
+namespace {
+int encode_swizzled_map(const void* base, int rank, const uint64_t* dims,
+                        const uint64_t* strides_bytes, const uint32_t* box,
+                        CUtensorMapDataType type, CUtensorMap* out) {
   if (rank < 2 || rank > 5) return set_error(B200_ERR_INVALID, "tensor map rank must be 2..5");
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0)
     return set_error(B200_ERR_INVALID, "tensor base must be 16-byte aligned");
   GenKey key{};
   key.base = base;
   key.rank = rank;
-  key.dtype = dtype;
+  key.dtype = static_cast<int>(type);
   for (int i = 0; i < rank; ++i) {
     key.dims[i] = dims[i];
     key.box[i] = box[i];
@@ -244,11 +245,8 @@ int encode_tensor_map_16b(const void* base, int rank, const uint64_t* dims,
   }
   CUtensorMap map;
   std::memset(&map, 0, sizeof(map));
-  const CUresult r = g_encode(&map,
-                              dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                              static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim, gstride,
-                              gbox, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUresult r = g_encode(&map, type, static_cast<cuuint32_t>(rank),
+                              const_cast<void*>(base), gdim, gstride, gbox, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -259,6 +257,23 @@ int encode_tensor_map_16b(const void* base, int rank, const uint64_t* dims,
   g_gen_maps.emplace(key, map);
   *out = map;
   return B200_OK;
+}
+
+}  // namespace
+
+int encode_tensor_map_16b(const void* base, int rank, const uint64_t* dims,
+                          const uint64_t* strides_bytes, const uint32_t* box, int dtype,
+                          CUtensorMap* out) {
+  return encode_swizzled_map(base, rank, dims, strides_bytes, box,
+                             dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                             out);
+}
+
+int encode_tensor_map_8b(const void* base, int rank, const uint64_t* dims,
+                         const uint64_t* strides_bytes, const uint32_t* box, CUtensorMap* out) {
+  return encode_swizzled_map(base, rank, dims, strides_bytes, box, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                             out);
 }
 
 }  // namespace b200

@@ -65,6 +65,10 @@ int encode_tensor_map_16b(const void* base, int rank, const uint64_t* dims,
                           const uint64_t* strides_bytes, const uint32_t* box, int dtype,
                           CUtensorMap* out);
 
+// The same for 8-bit elements.
+int encode_tensor_map_8b(const void* base, int rank, const uint64_t* dims,
+                         const uint64_t* strides_bytes, const uint32_t* box, CUtensorMap* out);
+
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Launch with programmatic stream serialization: the grid may be scheduled while

@@ -15,6 +15,9 @@ this module                            reference (``src/inferkernellab/``)
 ``build_slot_mapping``                 (new) device form of ``PagedKVCache.slot_mapping`` for a batch
 ``rope_append_kv``                     ``hf_benchmark._apply_rotary`` (:69-85) + ``append_kv_triton``
 ``paged_decode_attention_append``      (new) the append (+ rotary) above fused into the decode launch
+``qk_norm_rope_append``                (new) per-head RMS norm of q and k, rotary and append in one launch
+``copy_kv_pages``                      (new) pages copied to other pages in every layer
+``remap_block_tables``                 (new) block tables rewritten to new page ids
 ``add_rmsnorm`` / ``silu_mul``         (new) Transformers ``LlamaRMSNorm`` (+ residual add) and the
                                        ``act_fn(gate) * up`` of ``LlamaMLP``, one launch each
 =====================================  ==========================================================
@@ -486,6 +489,155 @@ def rope_append_kv(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         ctypes.byref(desc), ctypes.byref(args), query.data_ptr(), key.data_ptr(),
         value.data_ptr(), cos.data_ptr(), sin.data_ptr(), slots.data_ptr(), out.data_ptr(),
         _ERROR_WORDS.get(device).data_ptr(), _stream_ptr(device)))
+    return out
+
+
+def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                        q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                        sin: torch.Tensor, cache, slots: torch.Tensor, layer: int = 0, *,
+                        eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
+    """RMS norm of every q and k head, rotary embedding and K/V append in one launch.
+
+    For decoders with a norm on each query and key head: ``query`` ``[T, Hq, D]`` and ``key``
+    ``[T, Hkv, D]`` are normalised per head (``x * rsqrt(mean(x**2) + eps) * weight``, weights
+    ``[D]``), rotated as ``rope_append_kv`` does, and K and ``value`` are written to ``cache`` at
+    ``slots`` (negative: skipped).  ``cos``/``sin`` are ``[T, R]`` with an even ``R <= D``: the first
+    ``R`` dimensions are rotated, the others only normalised.  Everything is computed in 32 bits and
+    rounded once.  Returns the query (written to ``out`` when given).  Inputs may be strided views
+    whose last dimension is contiguous.
+    """
+    if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
+        raise ValueError("query must be [T, Hq, D] and key/value [T, Hkv, D]")
+    device = query.device
+    if device.type != "cuda" or any(t.device != device for t in (key, value, q_weight, k_weight,
+                                                                 cos, sin, slots)):
+        raise ValueError("all tensors must be on the same CUDA device")
+    layout = cache.layout
+    tokens, heads, dim = query.shape
+    if tuple(key.shape) != (tokens, layout.num_kv_heads, layout.head_dim) or dim != layout.head_dim:
+        raise ValueError("query/key/value shape does not match cache layout")
+    if heads % layout.num_kv_heads != 0:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    if q_weight.shape != (dim,) or k_weight.shape != (dim,):
+        raise ValueError("q_weight and k_weight must be [D]")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[0] != tokens:
+        raise ValueError("cos/sin must hold one row per token")
+    rotary = cos.shape[1]
+    if rotary <= 0 or rotary > dim or rotary % 2:
+        raise ValueError("the rotary dimension must be even and at most head_dim")
+    if slots.numel() != tokens:
+        raise ValueError("slots and query token counts must match")
+    if not 0 <= layer < layout.num_layers:
+        raise IndexError("layer is out of range")
+    if not eps >= 0.0:
+        raise ValueError("eps must be non-negative")
+    dtype = cache.k.dtype
+    if any(t.dtype != dtype for t in (query, key, value, q_weight, k_weight, cos, sin)):
+        raise ValueError("query/key/value/weights/cos/sin must have the cache dtype")
+    if slots.dtype not in _INDEX_CODE:
+        raise ValueError("slots must use int32 or int64")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+    elif (out.shape != query.shape or out.dtype != dtype or out.device != device
+          or out.stride(-1) != 1):
+        raise ValueError("out must match query's shape, dtype and device")
+    if tokens == 0:
+        return out
+    query, key, value, q_weight, k_weight, cos, sin = (
+        t if t.stride(-1) == 1 else t.contiguous()
+        for t in (query, key, value, q_weight, k_weight, cos, sin))
+    slots = slots.reshape(-1)
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    args = _lib.QkNormArgs(tokens, heads, layer, rotary, eps, *query.stride()[:2],
+                           *key.stride()[:2], *value.stride()[:2], *out.stride()[:2],
+                           cos.stride(0), sin.stride(0), _INDEX_CODE[slots.dtype])
+    desc = _cache_desc(cache)
+    _lib.check(_lib.load().b200_qk_norm_rope_append(
+        ctypes.byref(desc), ctypes.byref(args), query.data_ptr(), key.data_ptr(),
+        value.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
+        sin.data_ptr(), slots.data_ptr(), out.data_ptr(), _ERROR_WORDS.get(device).data_ptr(),
+        _stream_ptr(device)))
+    return out
+
+
+# --------------------------------------------------------------------- pages
+
+def copy_kv_pages(cache, src, dst, *, tokens=None) -> None:
+    """Copy physical pages ``src[i]`` to ``dst[i]`` in every layer of ``cache``, K and V, one launch.
+
+    ``tokens[i]`` limits pair ``i`` to its page's first tokens (a forked request's last, partly
+    filled page); by default whole pages are copied.  ``src``, ``dst`` and ``tokens`` are lists, or
+    int32/int64 tensors of one dtype on the cache's device.  Lists are checked: valid ids, no page
+    the destination of two pairs or a destination and a source.  Device tensors are not read on the
+    host: a negative id skips its pair, an id past the pool skips it and sets the device error word,
+    and pages that overlap as above end up with either content.
+    """
+    device = cache.k.device
+    if device.type != "cuda":
+        raise ValueError("the cache must live on a CUDA device")
+    layout = cache.layout
+    on_host = [v is None or isinstance(v, (list, tuple)) for v in (src, dst, tokens)]
+    if isinstance(src, (list, tuple)) and isinstance(dst, (list, tuple)):
+        if any(not 0 <= b < layout.num_blocks for b in (*src, *dst)):
+            raise ValueError("src/dst contain an invalid physical block id")
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("a page may be the destination of one copy only, and of none that "
+                             "reads it")
+    if isinstance(tokens, (list, tuple)) and any(not 0 <= n <= layout.block_size for n in tokens):
+        raise ValueError("tokens must lie in [0, block_size]")
+    given = [v for v in (src, dst, tokens) if v is not None]
+    if all(on_host):  # one copy to the device
+        if any(len(v) != len(src) for v in given):
+            raise ValueError("src, dst and tokens must have one entry per page")
+        given = list(torch.tensor([list(v) for v in given], dtype=torch.int32).to(device))
+    else:
+        dtypes = {v.dtype for v in given if isinstance(v, torch.Tensor)}
+        if len(dtypes) != 1 or not dtypes <= set(_INDEX_CODE):
+            raise ValueError("src, dst and tokens must share an int32/int64 dtype")
+        index = dtypes.pop()
+        given = [torch.tensor(v, dtype=index).to(device) if isinstance(v, (list, tuple)) else v
+                 for v in given]
+    if any(v.ndim != 1 or v.shape != given[0].shape for v in given):
+        raise ValueError("src, dst and tokens must have one entry per page")
+    if any(v.device != device for v in given):
+        raise ValueError("src, dst and tokens must be on the cache device")
+    given = [v if v.is_contiguous() else v.contiguous() for v in given]
+    desc = _cache_desc(cache)
+    _lib.check(_lib.load().b200_copy_kv_pages(
+        ctypes.byref(desc), given[0].data_ptr(), given[1].data_ptr(),
+        given[2].data_ptr() if tokens is not None else None, _INDEX_CODE[given[0].dtype],
+        given[0].numel(), _ERROR_WORDS.get(device).data_ptr(), _stream_ptr(device)))
+
+
+def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor, *,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """``page_map[block_tables]``: block tables rewritten to new page ids, one launch.
+
+    ``block_tables`` is int32/int64 ``[B, W]``, ``page_map`` int32 ``[num_blocks]`` (a page that
+    stays maps to itself).  Negative entries (unused columns) stay as they are; an entry past
+    ``page_map`` stays and sets the device error word.  ``out`` may be ``block_tables`` itself.
+    """
+    if block_tables.ndim != 2 or block_tables.device.type != "cuda":
+        raise ValueError("block_tables must be a 2-D CUDA tensor")
+    if block_tables.dtype not in _INDEX_CODE:
+        raise ValueError("block_tables must use int32 or int64")
+    if (page_map.ndim != 1 or page_map.dtype != torch.int32 or page_map.numel() == 0
+            or page_map.device != block_tables.device):
+        raise ValueError("page_map must be a 1-D int32 tensor on the tables' device")
+    if out is None:
+        out = torch.empty(block_tables.shape, dtype=block_tables.dtype, device=block_tables.device)
+    elif (out.shape != block_tables.shape or out.dtype != block_tables.dtype
+          or out.device != block_tables.device or (out.shape[1] > 1 and out.stride(1) != 1)):
+        raise ValueError("out must match block_tables, with contiguous rows")
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    page_map = page_map.contiguous()
+    _lib.check(_lib.load().b200_remap_block_tables(
+        block_tables.data_ptr(), _INDEX_CODE[block_tables.dtype], block_tables.stride(0),
+        block_tables.shape[0], block_tables.shape[1], page_map.data_ptr(), page_map.numel(),
+        out.data_ptr(), out.stride(0), _ERROR_WORDS.get(block_tables.device).data_ptr(),
+        _stream_ptr(block_tables.device)))
     return out
 
 
