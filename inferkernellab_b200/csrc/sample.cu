@@ -16,20 +16,22 @@
 // largest is never drawn.  The two log-probabilities use 32-bit weights, summed
 // per thread and joined in 64 bits.
 //
-// Layout.  A cluster of 1..8 CTAs owns a row and reads it from memory once: each
-// CTA keeps its slice in shared memory, first the logits, then the weights, and
-// everything that follows runs from there, with what the CTAs have to tell each
-// other read through distributed shared memory.  Warps own runs of neighbouring
-// tokens, so a prefix over warps is a prefix over indices.
+// Layout.  A cluster of 1..8 CTAs owns a row and reads it from memory once; each
+// CTA keeps its slice in shared memory as it came.  What the CTAs have to tell
+// each other is stored into the others' shared memory before a cluster barrier
+// and read locally after it.  Warps own runs of neighbouring tokens, so a prefix
+// over warps is a prefix over indices.
 //
-// Search.  Nothing is sorted.  The bits of w (w >= 0) are an order-preserving
-// key.  A histogram of counts and masses over 249 bins of an eighth of an
-// octave each finds the bin where the cut falls.  If at most kList tokens lie in
-// it (the usual case) they are gathered and the cut is resolved by counting, for
-// each of them, what precedes it.  Otherwise the bin is split into 1024 bins, as
-// often as it takes (equal weights at the end: the cut is then between indices).
-// The masses of a bin are kept as two 32-bit sums (low and high 16 bits; a CTA
-// holds at most 2^16 tokens), since 64-bit shared-memory atomics are loops.
+// Nothing that is as long as the vocabulary is sorted.  Without filters the masses
+// of the warps' runs name the run that holds the draw.  With filters few tokens
+// matter, and the threads' own largest tokens (known from the search for m) say
+// which: k of them above a bound prove that the first k tokens are above it, and
+// a mass of top_p among them proves the same of the top_p prefix.  The tokens
+// above that bound are gathered (kList at most), sorted in one CTA, cut, and
+// drawn from.  Where the bound leaves too many (a flat row, equal logits, a large
+// top_k), the cut is found by histograms of counts and masses over the bits of w
+// (w >= 0: they order like w), 1024 bins a level, until the bin's tokens fit the
+// list or are all equal, and the draw takes another pass over the slice.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -51,15 +53,23 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kList = 1024;      // tokens that are sorted
+constexpr int kFewTokens = 512;  // top_k up to which the threads' largest tokens bound the list
+// Bins of the threads' largest tokens: 11 per unit of (m - l) / T, so that 255 of
+// them span the weights above 2^-32; the last one holds everything below.
+constexpr int kCoarse = 256;
+constexpr float kCoarsePerUnit = 11.f;
+// Bins of the exact search.
 constexpr int kBins = 1024;
-constexpr int kFirstShift = 20;                         // bits below an eighth of an octave
-constexpr uint32_t kFirstBase = (127u - 31u) << 3;      // key >> 20 of w = 2^-31
+constexpr int kFirstShift = 20;                          // bits below an eighth of an octave
+constexpr uint32_t kFirstBase = (127u - 31u) << 3;       // key >> 20 of w = 2^-31
 constexpr int kFirstBins = (127 << 3) - kFirstBase + 1;  // 249: the last one holds w = 1
-constexpr int kList = 512;                              // tokens that are resolved by counting
-constexpr int kMaxSlice = 46 * 1024;                    // tokens of a CTA (184 KB of weights)
+constexpr int kMaxSlice = 46 * 1024;                     // tokens of a CTA
 constexpr float kLargest = 3.402823466e38f, kSmallest = 1.175494351e-38f;
+constexpr float kLog2e = 1.4426950408889634f;
 static_assert(kMaxSlice <= (1 << 16), "the 32-bit mass sums hold 2^16 tokens");
-static_assert(kList <= kThreads, "one thread per gathered token");
+static_assert(kList <= 2 * kThreads, "two list entries per thread");
+static_assert(kCoarse <= kThreads, "a thread per coarse bin");
 
 struct SampleParams {
   const void* logits;
@@ -77,60 +87,90 @@ struct SampleParams {
   int vocab, slice;
 };
 
-struct Cut {       // kept: key > cut.key, or key == cut.key and index <= cut.index
+struct Cut {  // kept: key > cut.key, or key == cut.key and index <= cut.index
   uint32_t key;
   int index;
+  u64 mass;  // of the kept tokens
 };
 
 struct Shared {
-  uint32_t count[2][kBins], low[2][kBins], high[2][kBins];  // the first histogram, the finer ones
-  uint2 list[2][kList];                                     // key, index (rank 0's is used)
-  int listed[2];
-  // What the other CTAs read, one slot per step.
-  float pub_max;
-  double pub_sum;
-  u64 pub_mass;
-  int pub_first, pub_pass;
-  u64 pub_warp_mass[kWarps];
-  float pub_warp_sum[kWarps];
-  int pub_warp_ties[kWarps];
-  int pub_tie_index;
+  u64 list[kList];  // rank 0: gathered tokens, key << 32 | ~index
+  // The threads' largest tokens: count, and mass in units of 2^-22.
+  uint32_t coarse_count[kCoarse], coarse_mass[kCoarse];
+  // The exact search: a bin's mass is two 32-bit sums (low and high 16 bits; a CTA
+  // holds at most 2^16 tokens), since 64-bit shared-memory atomics are loops.
+  uint32_t count[kBins], low[kBins], high[kBins];
+  // Written by every CTA of the cluster, read here after the next cluster barrier.
+  float max_of[kMaxCluster];
+  double sum_of[kMaxCluster];
+  int first_of[kMaxCluster], pass_of[kMaxCluster], listed_of[kMaxCluster];
+  u64 warp_mass[kMaxCluster * kWarps];
+  float warp_sum[kMaxCluster * kWarps];
+  int warp_ties[kMaxCluster * kWarps];
+  int listed[3];  // rank 0: list entries taken (first gathering, then one per search)
+  Cut cut;
   // Of this CTA alone.
-  uint2 local_list[kList];
-  u64 scan_mass[kWarps + 1];
-  uint32_t scan_count[kWarps + 1];
+  int local_first, local_listed;
   float red_f[kWarps];
   double red_d[kWarps];
-  u64 red_u[kWarps];
-  int red_i[kWarps], red_p[kWarps];
+  int red_i[kWarps];
+  u64 scan_mass[kWarps];
+  uint32_t scan_count[kWarps];
   int found_bin;
   uint32_t found_count, before_count;
-  u64 before_mass, found_mass;
-  Cut cut;
-  u64 cut_mass;
+  u64 before_mass;
+  int found;
 };
 
-static_assert(sizeof(Shared) + 16 + (kMaxSlice + 8) * 4 <= 227 * 1024, "shared memory of a CTA");
+constexpr int kSharedBytes = (static_cast<int>(sizeof(Shared)) + 15) / 16 * 16;
+static_assert(kSharedBytes + kMaxSlice * 4 <= 227 * 1024, "shared memory of a CTA");
 
+// 16 bytes of logits.
 template <typename L>
-__device__ __forceinline__ float logit_f32(L x);
-template <>
-__device__ __forceinline__ float logit_f32<float>(float x) {
-  return x;
-}
-template <>
-__device__ __forceinline__ float logit_f32<__half>(__half x) {
-  return __half2float(x);
-}
-template <>
-__device__ __forceinline__ float logit_f32<__nv_bfloat16>(__nv_bfloat16 x) {
-  return __bfloat162float(x);
-}
+struct Vec;
 
-__device__ __forceinline__ float no_nan(float x) { return x == x ? x : -INFINITY; }
+template <>
+struct Vec<float> {
+  static constexpr int kN = 4;
+  float4 v;
+  __device__ float get(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+  // NaN to -inf (the maximum of the two is the one that is a number); returns the largest.
+  __device__ float clean() {
+    v.x = fmaxf(v.x, -INFINITY);
+    v.y = fmaxf(v.y, -INFINITY);
+    v.z = fmaxf(v.z, -INFINITY);
+    v.w = fmaxf(v.w, -INFINITY);
+    return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+  }
+};
+
+template <typename L, typename L2>
+struct Vec16 {
+  static constexpr int kN = 8;
+  L2 v[4];
+  __device__ float get(int i) const {
+    return static_cast<float>(i % 2 ? v[i / 2].y : v[i / 2].x);
+  }
+  __device__ float clean() {
+    L2 low;
+    low.x = low.y = L(-INFINITY);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmax2(v[i], low);
+    const L2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(static_cast<float>(m.x), static_cast<float>(m.y));
+  }
+};
+
+template <>
+struct alignas(16) Vec<__half> : Vec16<__half, __half2> {};
+template <>
+struct alignas(16) Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {};
 
 __device__ __forceinline__ uint32_t mass_of(float w) {
   return __float2uint_rn(__fmul_rn(w, 2147483648.0f));
+}
+__device__ __forceinline__ uint32_t mass_of_key(uint32_t key) {
+  return mass_of(__uint_as_float(key));
 }
 
 template <typename V>
@@ -140,107 +180,377 @@ __device__ __forceinline__ V warp_sum(V v) {
   return v;
 }
 
-// Which measure a cut is made on.
-enum Measure { kCount, kMass };
+// Inclusive prefix over the lanes of a warp.
+template <typename V>
+__device__ __forceinline__ V warp_prefix(V v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
+enum Measure { kCount, kMass };  // what a cut is made on
 
 template <typename L>
 class Row {
  public:
-  __device__ Row(const SampleParams& p, Shared& s, float* w, cg::cluster_group cluster)
-      : p(p), s(s), w(w), cluster(cluster), ranks(cluster.num_blocks()),
-        rank(cluster.block_rank()), tid(threadIdx.x), warp(threadIdx.x >> 5),
-        lane(threadIdx.x & 31) {
-    first = rank * p.slice;
-    n = max(0, min(p.slice, p.vocab - first));
-    const int run = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
-    run0 = min(n, warp * run);
-    run1 = min(n, run0 + run);
-  }
+  using V = Vec<L>;
+  static constexpr int kN = V::kN;
+
+  __device__ Row(const SampleParams& p, Shared& s, V* raw, cg::cluster_group cluster)
+      : p(p), s(s), raw(raw), cluster(cluster), ranks(static_cast<int>(cluster.num_blocks())),
+        rank(static_cast<int>(cluster.block_rank())), tid(threadIdx.x), warp(threadIdx.x >> 5),
+        lane(threadIdx.x & 31) {}
 
   const SampleParams& p;
   Shared& s;
-  float* w;  // the slice: logits, then weights
+  V* raw;  // the slice, -inf past its end
   cg::cluster_group cluster;
-  const unsigned ranks, rank;
-  const int tid, warp, lane;
-  int first, n;    // the slice's first token and its length
-  int run0, run1;  // this warp's part of the slice
-  int level = 0;   // 0: the first histogram, 1: a finer one
-  int lists = 0;   // lists gathered so far (at most one per search)
+  const int ranks, rank, tid, warp, lane;
+  int origin;            // token of raw's first element
+  int run0, run1;        // this warp's vectors
+  float thread_max;      // largest logit of this thread's vectors
+  float m, inv, min_p;   // largest logit of the row, 1 / T
+  int searches = 0;
 
-  __device__ Shared* at(unsigned r) { return cluster.map_shared_rank(&s, r); }
+  __device__ Shared* at(int r) { return cluster.map_shared_rank(&s, r); }
 
-  // Reads the slice; returns the largest logit of the row (every thread).
-  __device__ float load(const L* row) {
-    constexpr int kVec = 16 / sizeof(L);
-    const L* src = row + first;
-    // 16-byte vectors from the first aligned element; w is shifted so that
-    // those elements are aligned in shared memory, too.
-    const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(src) / sizeof(L)) % kVec);
-    const int head = min(n, skip ? kVec - skip : 0);
-    w += skip;
-    const int vecs = (n - head) / kVec;
-    const int tail = head + vecs * kVec;
-    float m = -INFINITY;
-    if (tid < head) {
-      const float x = no_nan(logit_f32<L>(src[tid]));
-      w[tid] = x;
-      m = x;
-    }
-    if (tid < n - tail) {
-      const float x = no_nan(logit_f32<L>(src[tail + tid]));
-      w[tail + tid] = x;
-      m = fmaxf(m, x);
-    }
-    const uint4* vsrc = reinterpret_cast<const uint4*>(src + head);
-    float4* vdst = reinterpret_cast<float4*>(w + head);
-#pragma unroll 4
-    for (int i = tid; i < vecs; i += kThreads) {
-      const uint4 raw = vsrc[i];
-      L x[kVec];
-      memcpy(x, &raw, 16);
-      float f[kVec];
+  // ---------------------------------------------------------------- pass 1
+  // The vector that starts `skip` elements into `a` and ends in `b`.
+  __device__ static V shifted(const V& a, const V& b, int skip) {
+    uint32_t w[8], out[4];
+    memcpy(w, &a, 16);
+    memcpy(w + 4, &b, 16);
+    const int words = skip * static_cast<int>(sizeof(L)) / 4;
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        f[j] = no_nan(logit_f32<L>(x[j]));
-        m = fmaxf(m, f[j]);
+    for (int i = 0; i < 6; ++i) w[i] = words & 2 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = words & 1 ? w[i + 1] : w[i];
+    const int bits = sizeof(L) == 2 ? (skip & 1) * 16 : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    V x;
+    memcpy(&x, out, 16);
+    return x;
+  }
+
+  // Reads the slice into shared memory; sets m.
+  __device__ void load(const L* row) {
+    const int first = min(rank * p.slice, p.vocab);
+    const int n = min(p.slice, p.vocab - first);
+    const L* src = row + first;
+    const int vecs = (n + kN - 1) / kN;
+    origin = first;
+    const int run = ((vecs + kWarps - 1) / kWarps + 31) / 32 * 32;
+    run0 = min(vecs, warp * run);
+    run1 = min(vecs, run0 + run);
+    // A row off the 16-byte grid is read as two neighbouring vectors and shifted,
+    // so that a thread's tokens (and the rounding of its sum) do not depend on the
+    // address; vectors that reach past the slice on either side by element.
+    const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(src) / sizeof(L)) % kN);
+    const V* vsrc = reinterpret_cast<const V*>(src - skip);
+    const int whole0 = skip ? 1 : 0;
+    const int whole1 = skip ? (n + skip) / kN - 1 : n / kN;
+    thread_max = -INFINITY;
+    constexpr int kBatch = 4;  // loads in flight of a thread
+    for (int base = run0 + lane; base < run1; base += 32 * kBatch) {
+      V x[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int v = base + 32 * j;
+        if (v >= whole0 && v < min(whole1, run1)) x[j] = vsrc[v];
+      }
+      if (skip) {
+        V next[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int v = base + 32 * j;
+          if (v >= whole0 && v < min(whole1, run1)) next[j] = vsrc[v + 1];
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) x[j] = shifted(x[j], next[j], skip);
       }
 #pragma unroll
-      for (int j = 0; j < kVec / 4; ++j)
-        vdst[i * (kVec / 4) + j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+      for (int j = 0; j < kBatch; ++j) {
+        const int v = base + 32 * j;
+        if (v >= run1) break;
+        if (v < whole0 || v >= whole1) {
+          L e[kN];
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const int at = v * kN + i;
+            e[i] = at < n ? src[at] : static_cast<L>(-INFINITY);
+          }
+          memcpy(&x[j], e, 16);
+        }
+        thread_max = fmaxf(thread_max, x[j].clean());
+        raw[v] = x[j];
+      }
     }
+    m = thread_max;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s.red_f[warp] = m;
     __syncthreads();
-    if (tid == 0) {
+    if (tid < ranks) {
+      m = s.red_f[0];
       for (int i = 1; i < kWarps; ++i) m = fmaxf(m, s.red_f[i]);
-      s.pub_max = m;
+      at(tid)->max_of[rank] = m;
     }
     cluster.sync();
-    m = -INFINITY;
-    for (unsigned r = 0; r < ranks; ++r) m = fmaxf(m, at(r)->pub_max);
-    return m;
+    m = s.max_of[0];
+    for (int r = 1; r < ranks; ++r) m = fmaxf(m, s.max_of[r]);
   }
 
-  __device__ void clear_histogram(int bins) {
-    for (int i = tid; i < bins; i += kThreads)
-      s.count[level][i] = s.low[level][i] = s.high[level][i] = 0;
+  __device__ float argument(float l) const {  // of the exponential
+    return m == INFINITY ? (l == m ? 0.f : -INFINITY) : __fmul_rn(__fsub_rn(l, m), inv);
+  }
+  __device__ float weight(float l) const { return expf(argument(l)); }
+
+  __device__ static int coarse_bin(float x) {
+    return static_cast<int>(fminf(__fmul_rn(-x, kCoarsePerUnit), kCoarse - 1));
   }
 
-  __device__ void add_to_bin(int bin, uint32_t q, bool with_mass) {
-    atomicAdd(&s.count[level][bin], 1u);
-    if (with_mass) {
-      atomicAdd(&s.low[level][bin], q & 0xffffu);
-      atomicAdd(&s.high[level][bin], q >> 16);
+  // f(token, logit) for this warp's tokens in the slice's vectors.
+  template <typename F>
+  __device__ void each(F&& f) {
+#pragma unroll 2
+    for (int v = run0 + lane; v < run1; v += 32) {
+      const V x = raw[v];
+#pragma unroll
+      for (int i = 0; i < kN; ++i) f(origin + v * kN + i, x.get(i));
     }
+  }
+
+  // ---------------------------------------------------------------- pass 2
+  __device__ void push_sum(float sum) {
+    const double d = warp_sum(static_cast<double>(sum));
+    if (lane == 0) s.red_d[warp] = d;
+  }
+  __device__ void push_block_sums(bool exact, bool first) {
+    __syncthreads();
+    if (tid < ranks) {
+      double d = 0;
+      for (int i = 0; i < kWarps; ++i) d += s.red_d[i];
+      Shared* o = at(tid);
+      o->sum_of[rank] = d;
+      if (first) o->first_of[rank] = s.local_first;
+      if (exact) {
+        int pass = 0;
+        for (int i = 0; i < kWarps; ++i) pass += s.red_i[i];
+        // With min_p = 0 all tokens pass, and the padding after the slice would, too.
+        o->pass_of[rank] = min_p > 0.f ? pass : max(0, min(p.slice, p.vocab - rank * p.slice));
+      }
+    }
+  }
+  // The sum of w alone.  The 2-ulp exponential is enough for a logarithm's sake.
+  __device__ void sum_weights() {
+    const float c = fminf(inv * kLog2e, kLargest);
+    float sum = 0.f;
+    each([&](int, float l) { sum += fast_exp2((l - m) * c); });
+    push_sum(sum);
+  }
+  // The sum of w, and mass and number of the tokens that pass min_p, by warp.
+  __device__ void sum_masses() {
+    float sum = 0.f;
+    u64 mass = 0;
+    int pass = 0;
+    each([&](int, float l) {
+      const float w = weight(l);
+      sum += w;
+      if (w >= min_p) {
+        mass += mass_of(w);
+        ++pass;
+      }
+    });
+    push_sum(sum);
+    mass = warp_sum(mass);
+    pass = warp_sum(pass);
+    if (lane == 0) s.red_i[warp] = pass;
+    if (lane < ranks) at(lane)->warp_mass[rank * kWarps + warp] = mass;
+  }
+  __device__ void find_first_largest() {
+    if (thread_max == m)
+      each([&](int token, float l) {
+        if (l == m) atomicMin(&s.local_first, token);
+      });
+  }
+
+  // Mass of the first `warps` warps of the row (whole warps call it).
+  __device__ u64 mass_before(int warps) const {
+    u64 q = 0;
+    for (int i = lane; i < warps; i += 32) q += s.warp_mass[i];
+    return warp_sum(q);
+  }
+  __device__ u64 row_mass() const { return mass_before(ranks * kWarps); }
+  __device__ double row_sum() const {
+    double d = 0;
+    for (int r = 0; r < ranks; ++r) d += s.sum_of[r];
+    return d;
+  }
+
+  __device__ void add_coarse() {
+    if (thread_max == -INFINITY) return;
+    const float x = argument(thread_max);
+    const float w = expf(x);
+    if (!(w >= min_p)) return;
+    const int bin = coarse_bin(x);
+    atomicAdd(&s.coarse_count[bin], 1u);
+    atomicAdd(&s.coarse_mass[bin], mass_of(w) >> 9);
+  }
+
+  // The first coarse bin at which the threads' largest tokens of the row reach
+  // `target`, or -1.
+  __device__ int coarse_bound(Measure measure, u64 target) {
+    uint32_t c = 0;
+    if (tid < kCoarse)
+      for (int r = 0; r < ranks; ++r) {
+        const Shared* o = at(r);
+        c += measure == kCount ? o->coarse_count[tid] : o->coarse_mass[tid];
+        // 8 CTAs x 512 threads x 2^22: 33 bits; cap what only has to reach target
+        if (c > 0x7fffffffu) c = 0x7fffffffu;
+      }
+    u64 sum = warp_prefix(static_cast<u64>(c), lane);
+    if (lane == 31) s.scan_mass[warp] = sum;
+    if (tid == 0) s.found = -1;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) sum += s.scan_mass[i];
+    const u64 scale = measure == kCount ? 1 : 512;
+    if (tid < kCoarse && sum * scale >= target && (sum - c) * scale < target) s.found = tid;
+    __syncthreads();
+    return s.found;
+  }
+
+  // Every token above coarse bin `bound` that passes min_p to rank 0's list; true
+  // if they fit.  Has a cluster barrier.
+  __device__ bool gather(int bound) {
+    // A bound on l below the bin's edge by more than its rounding.
+    const float edge = (bound + 1) / kCoarsePerUnit / inv;
+    const float limit =
+        bound >= kCoarse - 1 ? -kLargest : m - edge * 1.0001f - (fabsf(m) + 1e-30f) * 1e-6f;
+    int mine = 0;
+    const bool any = thread_max >= limit;
+    if (any) each([&](int, float l) { mine += l >= limit; });
+    mine = warp_sum(mine);
+    if (lane == 0 && mine > 0) atomicAdd(&s.local_listed, mine);
+    __syncthreads();
+    const int total = s.local_listed;
+    if (any && total <= kList) {
+      Shared* home = at(0);
+      each([&](int token, float l) {
+        if (l >= limit) {
+          const float w = weight(l);
+          if (w >= min_p && w > 0.f) {
+            const int to = atomicAdd(&home->listed[0], 1);
+            if (to < kList) home->list[to] = entry(w, token);
+          }
+        }
+      });
+    }
+    if (tid < ranks) at(tid)->listed_of[rank] = total;
+    cluster.sync();
+    int sum = 0;
+    for (int r = 0; r < ranks; ++r) sum += s.listed_of[r];
+    return sum <= kList;
+  }
+
+  __device__ static u64 entry(float w, int token) {
+    return static_cast<u64>(__float_as_uint(w)) << 32 | static_cast<uint32_t>(~token);
+  }
+
+  // ------------------------------------------------------------- the list
+  // Sorts the first n list entries, largest first (rank 0; the rest is cleared).
+  __device__ void sort_list(int n) {
+    int size = 2;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
+    __syncthreads();
+    const bool small = size <= 64;  // one warp, two entries a lane
+    if (!small || warp == 0) {
+      for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+          if (tid < size / 2) {
+            const int a = 2 * tid - (tid & (j - 1)), b = a + j;
+            const u64 x = s.list[a], y = s.list[b];
+            if ((x < y) == ((a & k) == 0)) {
+              s.list[a] = y;
+              s.list[b] = x;
+            }
+          }
+          if (small)
+            __syncwarp();
+          else
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+  }
+
+  // The position among the first n list entries at which the running measure,
+  // on top of `before`, reaches target (n: it does not); *sum gets the mass of
+  // the entries up to and with it.  key_shift: where an entry holds its key.
+  __device__ int list_position(int n, int key_shift, Measure measure, u64 before, u64 target,
+                               u64 before_mass, u64* sum) {
+    u64 q[2], c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = 2 * tid + i;
+      q[i] = at < n ? mass_of_key(static_cast<uint32_t>(s.list[at] >> key_shift)) : 0;
+      c[i] = measure == kMass ? q[i] : (at < n ? 1 : 0);
+    }
+    u64 mass = warp_prefix(q[0] + q[1], lane);
+    if (lane == 31) s.scan_mass[warp] = mass;
+    if (tid == 0) s.found = n;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) mass += s.scan_mass[i];
+    mass -= q[0] + q[1];  // before this thread
+    u64 run = before + (measure == kMass ? mass : static_cast<u64>(min(n, 2 * tid)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mass += q[i];
+      if (run < target && run + c[i] >= target) {
+        s.found = 2 * tid + i;
+        s.before_mass = before_mass + mass;
+      }
+      run += c[i];
+    }
+    __syncthreads();
+    const int found = s.found;
+    if (sum && found < n) *sum = s.before_mass;
+    __syncthreads();
+    return found;
+  }
+
+  __device__ u64 list_mass(int n) {
+    u64 q = 0;
+    for (int i = tid; i < n; i += kThreads) q += mass_of_key(static_cast<uint32_t>(s.list[i] >> 32));
+    q = warp_sum(q);
+    if (lane == 0) s.scan_mass[warp] = q;
+    __syncthreads();
+    q = 0;
+    for (int i = 0; i < kWarps; ++i) q += s.scan_mass[i];
+    __syncthreads();
+    return q;
+  }
+
+  // --------------------------------------------------------- exact search
+  __device__ void clear_histogram() {
+    for (int i = tid; i < kBins; i += kThreads) s.count[i] = s.low[i] = s.high[i] = 0;
+    __syncthreads();
+  }
+  __device__ void add_to_bin(int bin, uint32_t q) {
+    atomicAdd(&s.count[bin], 1u);
+    atomicAdd(&s.low[bin], q & 0xffffu);
+    atomicAdd(&s.high[bin], q >> 16);
   }
 
   // The bin of the row's histogram in which `target` is reached, counted from the
   // last bin down, on top of `count0` / `mass0` above the whole histogram; bin 0
-  // of the first histogram is given by what the row's totals leave.  Sets
-  // s.found_bin (-1: the row has less than target), found_count / found_mass (of
-  // the bin) and before_count / before_mass (above it).
+  // of the first level is what the row's totals leave.  Sets s.found_bin (-1: the
+  // row has less than target), found_count (of the bin) and before_count /
+  // before_mass (above it).
   __device__ void find_bin(int bins, Measure measure, u64 target, uint32_t count0, u64 mass0,
                            bool first_level, uint32_t row_count, u64 row_mass) {
     if (tid == 0) s.found_bin = -1;
@@ -253,26 +563,16 @@ class Row {
       u64 q = 0;
       if (bin >= (first_level ? 1 : 0)) {
         u64 lo = 0, hi = 0;
-        for (unsigned r = 0; r < ranks; ++r) {
+        for (int r = 0; r < ranks; ++r) {
           const Shared* o = at(r);
-          c += o->count[level][bin];
-          lo += o->low[level][bin];
-          hi += o->high[level][bin];
+          c += o->count[bin];
+          lo += o->low[bin];
+          hi += o->high[bin];
         }
         q = lo + (hi << 16);
       }
-      // Inclusive prefix over the block.
-      uint32_t ci = c;
-      u64 qi = q;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t cu = __shfl_up_sync(0xffffffffu, ci, o);
-        const u64 qu = __shfl_up_sync(0xffffffffu, qi, o);
-        if (lane >= o) {
-          ci += cu;
-          qi += qu;
-        }
-      }
+      uint32_t ci = warp_prefix(c, lane);
+      u64 qi = warp_prefix(q, lane);
       if (lane == 31) {
         s.scan_count[warp] = ci;
         s.scan_mass[warp] = qi;
@@ -288,8 +588,8 @@ class Row {
         total_c += s.scan_count[i];
         total_q += s.scan_mass[i];
       }
-      uint32_t before_c = run_count + ci - c;
-      u64 before_q = run_mass + qi - q;
+      const uint32_t before_c = run_count + ci - c;
+      const u64 before_q = run_mass + qi - q;
       if (first_level && bin == 0) {  // what the bins above leave of the row
         c = row_count - before_c;
         q = row_mass - before_q;
@@ -300,7 +600,6 @@ class Row {
         if (before < target && target <= with) {
           s.found_bin = bin;
           s.found_count = c;
-          s.found_mass = q;
           s.before_count = before_c;
           s.before_mass = before_q;
         }
@@ -313,300 +612,350 @@ class Row {
   }
 
   // The cut of the prefix that reaches `target` (>= 1): tokens up to and with the
-  // one whose inclusive measure reaches it.  Returns false if all tokens with
-  // w >= floor_w together have less; else sets s.cut and s.cut_mass (mass kept,
-  // meaningful if the histograms carry masses).  The first histogram is in place
-  // (buffer 0) and visible to the cluster.
-  __device__ bool cut_at(Measure measure, u64 target, bool with_mass, float floor_w,
-                         uint32_t row_count, u64 row_mass) {
-    level = 0;
+  // one whose inclusive measure reaches it, into s.cut.  False if all tokens that
+  // pass min_p together have less.
+  __device__ bool cut_at(Measure measure, u64 target, uint32_t row_count, u64 row_mass) {
+    clear_histogram();
+    each([&](int, float l) {
+      const float w = weight(l);
+      const uint32_t hi = __float_as_uint(w) >> kFirstShift;
+      if (hi > kFirstBase && w >= min_p) add_to_bin(hi - kFirstBase, mass_of(w));
+    });
+    cluster.sync();
     find_bin(kFirstBins, measure, target, 0, 0, true, row_count, row_mass);
+    cluster.sync();  // the histograms may be cleared again
     if (s.found_bin < 0) return false;
     uint32_t lo = s.found_bin == 0 ? 0u : (kFirstBase + s.found_bin) << kFirstShift;
     uint32_t size = s.found_bin == 0 ? (kFirstBase + 1) << kFirstShift : 1u << kFirstShift;
-    const uint32_t floor_key = __float_as_uint(floor_w);
     while (s.found_count > kList && size > 1) {
-      const int shift = size > (1u << kFirstShift) ? kFirstShift : (size > 1024u ? 10 : 0);
+      const int shift = size > (1u << kFirstShift) ? kFirstShift : (size > kBins ? 10 : 0);
       const int bins = static_cast<int>((size + (1u << shift) - 1) >> shift);
       const uint32_t before_count = s.before_count;
       const u64 before_mass = s.before_mass;
-      level = 1;  // its last readers have passed the cluster barrier at the end of this loop
-      clear_histogram(kBins);
-      __syncthreads();
-      for (int i = run0 + lane; i < run1; i += 32) {
-        const float x = w[i];
-        const uint32_t key = __float_as_uint(x);
-        if (key - lo < size && key >= floor_key) add_to_bin((key - lo) >> shift, mass_of(x), true);
-      }
+      clear_histogram();
+      each_in(lo, size, [&](int, uint32_t key) {
+        add_to_bin(static_cast<int>((key - lo) >> shift), mass_of_key(key));
+      });
       cluster.sync();
+      // The totals above are exact, so one of these bins holds the target.
       find_bin(bins, measure, target, before_count, before_mass, false, 0, 0);
-      // Totals of the bin above are exact, so one of its bins holds the target.
-      if (s.found_bin < 0) return false;
+      cluster.sync();
       lo += static_cast<uint32_t>(s.found_bin) << shift;
       size = 1u << shift;
-      cluster.sync();
     }
-    if (s.found_count <= kList) {
-      resolve_listed(measure, target, lo, size, floor_key);
-    } else {
+    if (s.found_count <= kList)
+      resolve_listed(measure, target, lo, size);
+    else
       resolve_ties(measure, target, lo);
-    }
     return true;
   }
 
-  // At most kList tokens with keys in [lo, lo + size): all of them to every CTA,
-  // one thread each, and the one that reaches the target is the cut.
-  __device__ void resolve_listed(Measure measure, u64 target, uint32_t lo, uint32_t size,
-                                 uint32_t floor_key) {
-    const int slot = lists++;
+  // f(token, key) for the tokens that pass min_p with keys in [lo, lo + size).
+  template <typename F>
+  __device__ void each_in(uint32_t lo, uint32_t size, F&& f) {
+    each([&](int token, float l) {
+      const float w = weight(l);
+      const uint32_t key = __float_as_uint(w);
+      if (key - lo < size && w >= min_p && in_slice(token)) f(token, key);
+    });
+  }
+  __device__ bool in_slice(int token) const {  // false for the padding after it
+    return token < min(p.vocab, (rank + 1) * p.slice);
+  }
+
+  // At most kList tokens with keys in [lo, lo + size): sorted by rank 0.
+  __device__ void resolve_listed(Measure measure, u64 target, uint32_t lo, uint32_t size) {
+    const int slot = 1 + searches;
+    const u64 before_mass = s.before_mass;
+    const u64 before = measure == kCount ? s.before_count : before_mass;
     Shared* home = at(0);
-    for (int i = run0 + lane; i < run1; i += 32) {
-      const uint32_t key = __float_as_uint(w[i]);
-      if (key - lo < size && key >= floor_key) {
-        const int to = atomicAdd(&home->listed[slot], 1);
-        if (to < kList) home->list[slot][to] = make_uint2(key, static_cast<uint32_t>(first + i));
+    each_in(lo, size, [&](int token, uint32_t key) {
+      const int to = atomicAdd(&home->listed[slot], 1);
+      if (to < kList) home->list[to] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~token);
+    });
+    cluster.sync();
+    if (rank == 0) {
+      const int n = min(s.listed[slot], kList);
+      sort_list(n);
+      Cut cut = {0, 0x7fffffff, 0};
+      const int pos = list_position(n, 32, measure, before, target, before_mass, &cut.mass);
+      if (pos < n) {
+        cut.key = static_cast<uint32_t>(s.list[pos] >> 32);
+        cut.index = static_cast<int>(~static_cast<uint32_t>(s.list[pos]));
       }
+      if (tid < ranks) at(tid)->cut = cut;
     }
     cluster.sync();
-    const int m = min(home->listed[slot], kList);
-    if (tid < m) s.local_list[tid] = home->list[slot][tid];
-    __syncthreads();
-    if (tid < m) {
-      const uint2 me = s.local_list[tid];
-      const uint32_t mine = mass_of(__uint_as_float(me.x));
-      u64 c = s.before_count, q = s.before_mass;
-      for (int j = 0; j < m; ++j) {
-        const uint2 o = s.local_list[j];
-        if (o.x > me.x || (o.x == me.x && o.y < me.y)) {
-          ++c;
-          q += mass_of(__uint_as_float(o.x));
-        }
-      }
-      const u64 before = measure == kCount ? c : q;
-      const u64 with = before + (measure == kCount ? 1u : mine);
-      if (before < target && target <= with) {
-        s.cut.key = me.x;
-        s.cut.index = static_cast<int>(me.y);
-        s.cut_mass = q + mine;
-      }
-    }
-    __syncthreads();
   }
 
   // More than kList tokens of one and the same weight: the cut is the r-th of them
   // in order of index.
   __device__ void resolve_ties(Measure measure, u64 target, uint32_t key) {
-    const uint32_t q = mass_of(__uint_as_float(key));
+    const uint32_t q = mass_of_key(key);
     const u64 r = measure == kCount ? target - s.before_count
                                     : (target - s.before_mass + q - 1) / max(q, 1u);
+    const Cut found = {key, 0, s.before_mass + r * q};
     int ties = 0;
-    for (int i = run0 + lane; i < run1; i += 32) ties += __float_as_uint(w[i]) == key;
+    each_in(key, 1, [&](int, uint32_t) { ++ties; });
     ties = warp_sum(ties);
-    if (lane == 0) s.pub_warp_ties[warp] = ties;
-    if (tid == 0) s.pub_tie_index = -1;
+    if (lane < ranks) at(lane)->warp_ties[rank * kWarps + warp] = ties;
     cluster.sync();
     u64 before = 0;
-    for (unsigned o = 0; o < rank; ++o)
-      for (int i = 0; i < kWarps; ++i) before += at(o)->pub_warp_ties[i];
-    for (int i = 0; i < warp; ++i) before += s.pub_warp_ties[i];
+    for (int i = 0; i < rank * kWarps + warp; ++i) before += s.warp_ties[i];
     if (before < r && r <= before + ties) {  // warp-uniform: the r-th is in this run
-      for (int base = run0; base < run1; base += 32) {
-        const int i = base + lane;
-        const bool tie = i < run1 && __float_as_uint(w[i]) == key;
-        const unsigned vote = __ballot_sync(0xffffffffu, tie);
-        const u64 here = before + __popc(vote & ((2u << lane) - 1u));
-        if (tie && here == r) s.pub_tie_index = first + i;
-        before += __popc(vote);
-      }
+      walk(before, [&](int token, float l) {
+        const float w = weight(l);
+        return static_cast<u64>(__float_as_uint(w) == key && w >= min_p && in_slice(token));
+      }, r - 1, [&](int token) {
+        Cut cut = found;
+        cut.index = token;
+        for (int o = 0; o < ranks; ++o) at(o)->cut = cut;
+      });
     }
     cluster.sync();
-    int index = -1;
-    for (unsigned o = 0; o < ranks; ++o) index = max(index, at(o)->pub_tie_index);
-    if (tid == 0) {
-      s.cut.key = key;
-      s.cut.index = index;
-      s.cut_mass = s.before_mass + r * q;
-    }
-    __syncthreads();
   }
 
+  // Walks this warp's run in order of index, adding value(token, logit) to
+  // `running`; done(token) is called by one lane for the first token that takes it
+  // past t.
+  template <typename F, typename G>
+  __device__ void walk(u64 running, F&& value, u64 t, G&& done) {
+    for (int v = run0; v < run1; v += 32) {
+      const bool live = v + lane < run1;
+      u64 q[kN], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        q[i] = live ? value(origin + (v + lane) * kN + i, raw[v + lane].get(i)) : 0;
+        sum += q[i];
+      }
+      const u64 with = running + warp_prefix(sum, lane);
+      const unsigned vote = __ballot_sync(0xffffffffu, with > t);
+      if (vote) {
+        if (lane == __ffs(vote) - 1) {
+          u64 before = with - sum;
+          int token = 0;
+          bool open = true;
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            before += q[i];
+            if (open && before > t) {
+              token = origin + (v + lane) * kN + i;
+              open = false;
+            }
+          }
+          done(token);
+        }
+        return;
+      }
+      running = __shfl_sync(0xffffffffu, with, 31);
+    }
+  }
+
+  // ------------------------------------------------------------- the draw
+  __device__ static u64 draw_target(float u, u64 total) {
+    // u outside [0, 1) is taken as the nearest end
+    const double at = floor(static_cast<double>(u > 0.f ? u : 0.f) * static_cast<double>(total));
+    const u64 t = static_cast<u64>(at);
+    return t < total ? t : total - 1;
+  }
+
+  // One thread of the cluster writes the row's results.
+  __device__ void write(long long b, int token, const L* logits, double sum, double kept) {
+    const double x = argument(fmaxf(static_cast<float>(logits[token]), -INFINITY));
+    p.tokens[b] = token;
+    p.logprobs[b] = static_cast<float>(x - log(sum));
+    p.sampling_logprobs[b] = static_cast<float>(x - log(kept));
+  }
+
+  // The token at mass t of the row, whose warps' masses are in place.
+  template <typename F>
+  __device__ void draw(float u, F&& value, long long b, const L* logits, double sum, double kept) {
+    const u64 t = draw_target(u, row_mass());
+    const int me = rank * kWarps + warp;
+    const u64 before = mass_before(me);
+    if (before <= t && t < before + s.warp_mass[me])  // warp-uniform
+      walk(before, value, t, [&](int token) { write(b, token, logits, sum, kept); });
+  }
 };
 
 template <typename L>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
-  float* w_base = reinterpret_cast<float*>(smem + (sizeof(Shared) + 15) / 16 * 16);
   cg::cluster_group cluster = cg::this_cluster();
-  Row<L> row(p, s, w_base, cluster);
-  const int tid = row.tid, warp = row.warp, lane = row.lane;
+  Row<L> row(p, s, reinterpret_cast<Vec<L>*>(smem + kSharedBytes), cluster);
+  const int tid = row.tid, warp = row.warp, lane = row.lane, rank = row.rank;
   const long long b = blockIdx.x / row.ranks;
-  row.clear_histogram(kFirstBins);
+  if (tid < kCoarse) s.coarse_count[tid] = s.coarse_mass[tid] = 0;
   if (tid == 0) {
-    s.listed[0] = s.listed[1] = 0;
-    s.pub_first = p.vocab;
+    s.listed[0] = s.listed[1] = s.listed[2] = s.local_listed = 0;
+    s.local_first = p.vocab;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const L* logits = reinterpret_cast<const L*>(p.logits) + b * p.stride;
   const float temperature = p.temperature ? p.temperature[b] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
-  float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
-  int top_k = p.top_k ? p.top_k[b] : p.top_k_all;
+  const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
+  const int top_k = p.top_k ? p.top_k[b] : p.top_k_all;
   const float u = p.uniforms[b];
   const bool greedy = !(temperature > 0.f);
   const bool cut_k = top_k > 0 && top_k < p.vocab;
   const bool cut_p = top_p < 1.f;
-  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+  row.min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
   // Finite and not zero, so that 0 and -inf keep their meaning when multiplied.
-  const float inv = greedy ? 1.f : fmaxf(fminf(__fdiv_rn(1.f, temperature), kLargest), kSmallest);
+  row.inv = greedy ? 1.f : fmaxf(fminf(__fdiv_rn(1.f, temperature), kLargest), kSmallest);
+  const bool filtered = cut_k || cut_p || row.min_p > 0.f;
 
-  const float m = row.load(logits);
-  if (m == -INFINITY) {  // cluster-uniform: nothing in this row can be drawn
-    if (row.rank == 0 && tid == 0) {
+  row.load(logits);
+  if (row.m == -INFINITY) {  // cluster-uniform: nothing in this row can be drawn
+    if (rank == 0 && tid == 0) {
       p.tokens[b] = -1;
       p.logprobs[b] = -INFINITY;
       p.sampling_logprobs[b] = -INFINITY;
     }
-    cluster.sync();  // no CTA leaves while another may still read its pub_max
+    return;
+  }
+  // Whether the threads' largest tokens can bound what has to be gathered.
+  const bool few = cut_k && top_k <= kFewTokens;
+  const bool listing = filtered && row.m != INFINITY && (few || !cut_k);
+  // The masses of all tokens: to draw from, or for top_p of them.
+  bool exact = filtered ? !listing || (cut_p && !few) : !greedy || row.m == INFINITY;
+  if (listing && (few || cut_p)) row.add_coarse();
+  if (exact)
+    row.sum_masses();
+  else
+    row.sum_weights();
+  if (greedy) row.find_first_largest();
+  row.push_block_sums(exact, greedy);
+  cluster.sync();
+  const double sum = row.row_sum();
+  int first = p.vocab;
+  if (greedy)
+    for (int r = 0; r < row.ranks; ++r) first = min(first, s.first_of[r]);
+  if (!filtered) {
+    if (!greedy)
+      row.draw(u, [&](int, float l) { return static_cast<u64>(mass_of(row.weight(l))); }, b, logits,
+               sum, sum);
+    else if (rank == 0 && tid == 0)
+      row.write(b, first, logits, sum, sum);
     return;
   }
 
-  // Weights, their sums and the first histogram.
-  float* w = row.w;
-  float sum = 0.f;
-  u64 mass = 0;
-  int pass = 0;
-  for (int i = row.run0 + lane; i < row.run1; i += 32) {
-    const float l = w[i];
-    const float x = m == INFINITY ? (l == m ? 0.f : -INFINITY) : __fmul_rn(__fsub_rn(l, m), inv);
-    const float e = expf(x);
-    w[i] = e;
-    sum += e;
-    if (l == m) atomicMin(&s.pub_first, row.first + i);
-    if (e >= min_p) {
-      const uint32_t q = mass_of(e);
-      mass += q;
-      ++pass;
+  auto top_p_target = [&](u64 mass) {
+    const double t = ceil(static_cast<double>(top_p) * static_cast<double>(mass));
+    return t >= 1.0 ? static_cast<u64>(t) : 1ull;
+  };
+  if (listing) {
+    int bound = kCoarse - 1;  // every token
+    if (p.vocab > kList) {
+      if (few) {
+        bound = row.coarse_bound(kCount, static_cast<u64>(top_k));
+        if (bound < 0) bound = kCoarse - 1;
+      } else if (cut_p) {
+        bound = row.coarse_bound(kMass, top_p_target(row.row_mass()));
+      } else {
+        bound = min(kCoarse - 1, Row<L>::coarse_bin(logf(row.min_p)) + 1);
+      }
+    }
+    if (bound >= 0 && row.gather(bound)) {  // cluster-uniform
+      if (rank != 0) return;
+      const int n = s.listed[0];
+      int kept = n;
       if (cut_k || cut_p) {
-        const uint32_t hi = __float_as_uint(e) >> kFirstShift;
-        if (hi > kFirstBase) row.add_to_bin(hi - kFirstBase, q, cut_p);
+        row.sort_list(n);
+        if (cut_k) kept = min(n, top_k);
+        if (cut_p) {
+          const u64 mass = few ? row.list_mass(kept) : row.row_mass();
+          const int pos = row.list_position(kept, 32, kMass, 0, top_p_target(mass), 0, nullptr);
+          kept = min(kept, pos + 1);
+        }
       }
-    }
-  }
-  double dsum = warp_sum(static_cast<double>(sum));
-  mass = warp_sum(mass);
-  pass = warp_sum(pass);
-  if (lane == 0) {
-    s.red_d[warp] = dsum;
-    s.red_u[warp] = mass;
-    s.red_p[warp] = pass;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kWarps; ++i) {
-      dsum += s.red_d[i];
-      mass += s.red_u[i];
-      pass += s.red_p[i];
-    }
-    s.pub_sum = dsum;
-    s.pub_mass = mass;
-    s.pub_pass = pass;
-  }
-  cluster.sync();
-  double row_sum = 0;
-  u64 row_mass = 0;
-  uint32_t row_pass = 0;
-  int row_first = p.vocab;
-  for (unsigned r = 0; r < row.ranks; ++r) {
-    const Shared* o = row.at(r);
-    row_sum += o->pub_sum;
-    row_mass += o->pub_mass;
-    row_pass += o->pub_pass;
-    row_first = min(row_first, o->pub_first);
-  }
-
-  // The cut: top_k first, then top_p of the mass that is left.
-  Cut cut = {__float_as_uint(min_p), 0x7fffffff};
-  u64 left = row_mass;
-  if (cut_k && row.cut_at(kCount, static_cast<u64>(top_k), cut_p, min_p, row_pass, row_mass)) {
-    cut = s.cut;
-    left = s.cut_mass;
-  }
-  if (cut_p) {
-    const double t = ceil(static_cast<double>(top_p) * static_cast<double>(left));
-    const u64 target = t >= 1.0 ? static_cast<u64>(t) : 1ull;
-    __syncthreads();  // s.cut and s.found_* of the first search have been read
-    if (row.cut_at(kMass, target, true, min_p, row_pass, row_mass)) cut = s.cut;
-  }
-
-  // Kept mass and sum of every warp's run.
-  u64 kept_mass = 0;
-  float kept_sum = 0.f;
-  for (int i = row.run0 + lane; i < row.run1; i += 32) {
-    const float e = w[i];
-    const uint32_t key = __float_as_uint(e);
-    if (key > cut.key || (key == cut.key && row.first + i <= cut.index)) {
-      kept_mass += mass_of(e);
-      kept_sum += e;
-    }
-  }
-  kept_mass = warp_sum(kept_mass);
-  kept_sum = warp_sum(kept_sum);
-  if (lane == 0) {
-    s.pub_warp_mass[warp] = kept_mass;
-    s.pub_warp_sum[warp] = kept_sum;
-  }
-  cluster.sync();
-  u64 total = 0, before = 0;
-  double sampling_sum = 0;
-  for (unsigned r = 0; r < row.ranks; ++r) {
-    const Shared* o = row.at(r);
-    for (int i = 0; i < kWarps; ++i) {
-      if (r == row.rank && i == warp) before = total;
-      total += o->pub_warp_mass[i];
-      sampling_sum += o->pub_warp_sum[i];
-    }
-  }
-  const double at = floor(static_cast<double>(u > 0.f ? u : 0.f) * static_cast<double>(total));
-  u64 t = static_cast<u64>(at);
-  if (t >= total) t = total - 1;
-  int token = -1;
-  if (greedy) {
-    if (row.rank == 0 && warp == 0) token = row_first;
-  } else if (before <= t && t < before + kept_mass) {  // warp-uniform
-    for (int base = row.run0; base < row.run1 && token < 0; base += 32) {
-      const int i = base + lane;
-      uint32_t q = 0;
-      if (i < row.run1) {
-        const float e = w[i];
-        const uint32_t key = __float_as_uint(e);
-        if (key > cut.key || (key == cut.key && row.first + i <= cut.index)) q = mass_of(e);
-      }
-      u64 sums = q;
+      // The kept tokens by index, and their sum.
+      double kept_sum = 0;
+      u64 e[2];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 up = __shfl_up_sync(0xffffffffu, sums, o);
-        if (lane >= o) sums += up;
+      for (int i = 0; i < 2; ++i) {
+        const int at = tid + i * kThreads;
+        e[i] = at < kept ? s.list[at] : 0;
+        kept_sum += __uint_as_float(static_cast<uint32_t>(e[i] >> 32));
       }
-      const unsigned vote = __ballot_sync(0xffffffffu, before + sums > t);
-      if (vote) token = row.first + base + __ffs(vote) - 1;
-      before += __shfl_sync(0xffffffffu, sums, 31);
+      const u64 total = row.list_mass(kept);
+      kept_sum = warp_sum(kept_sum);
+      if (lane == 0) s.red_d[warp] = kept_sum;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = tid + i * kThreads;
+        if (at < kept) s.list[at] = e[i] << 32 | e[i] >> 32;  // ~index above the key
+      }
+      __syncthreads();
+      kept_sum = 0;
+      for (int i = 0; i < kWarps; ++i) kept_sum += s.red_d[i];
+      if (greedy) {
+        if (tid == 0) row.write(b, first, logits, sum, kept_sum);
+        return;
+      }
+      row.sort_list(kept);
+      const int pos = row.list_position(kept, 0, kMass, 0, Row<L>::draw_target(u, total) + 1, 0,
+                                        nullptr);
+      if (tid == 0)
+        row.write(b, static_cast<int>(~static_cast<uint32_t>(s.list[pos] >> 32)), logits, sum,
+                  kept_sum);
+      return;
     }
   }
-  if (token >= 0 && lane == 0) {
-    const float l = no_nan(logit_f32<L>(logits[token]));
-    const double x = m == INFINITY ? 0.0 : static_cast<double>(__fmul_rn(__fsub_rn(l, m), inv));
-    p.tokens[b] = token;
-    p.logprobs[b] = static_cast<float>(x - log(row_sum));
-    p.sampling_logprobs[b] = static_cast<float>(x - log(sampling_sum));
+
+  // Too many tokens for the list: exact cuts, then a draw over the slices.
+  if (!exact) {
+    __syncthreads();
+    row.sum_masses();
+    row.push_block_sums(true, false);
+    cluster.sync();
   }
-  cluster.sync();  // no CTA leaves while another may still read its shared memory
+  uint32_t pass = 0;
+  for (int r = 0; r < row.ranks; ++r) pass += s.pass_of[r];
+  const u64 mass = row.row_mass();
+  Cut cut = {__float_as_uint(row.min_p), 0x7fffffff, mass};
+  if (cut_k && row.cut_at(kCount, static_cast<u64>(top_k), pass, mass)) cut = s.cut;
+  if (cut_p) {
+    ++row.searches;
+    __syncthreads();  // s.cut has been read
+    if (row.cut_at(kMass, top_p_target(cut.mass), pass, mass)) cut = s.cut;
+  }
+  auto kept_weight = [&](int token, float l) {
+    const float w = row.weight(l);
+    const uint32_t key = __float_as_uint(w);
+    return key > cut.key || (key == cut.key && token <= cut.index) ? w : 0.f;
+  };
+  u64 kept_mass = 0;
+  float kept_part = 0.f;
+  row.each([&](int token, float l) {
+    const float w = kept_weight(token, l);
+    kept_mass += mass_of(w);
+    kept_part += w;
+  });
+  kept_mass = warp_sum(kept_mass);
+  kept_part = warp_sum(kept_part);
+  cluster.sync();  // every warp_mass has been read
+  if (lane < row.ranks) {
+    Shared* o = row.at(lane);
+    o->warp_mass[rank * kWarps + warp] = kept_mass;
+    o->warp_sum[rank * kWarps + warp] = kept_part;
+  }
+  cluster.sync();
+  double kept = 0;
+  for (int i = lane; i < row.ranks * kWarps; i += 32) kept += s.warp_sum[i];
+  kept = warp_sum(kept);
+  if (greedy) {
+    if (rank == 0 && tid == 0) row.write(b, first, logits, sum, kept);
+    return;
+  }
+  row.draw(u, [&](int token, float l) { return static_cast<u64>(mass_of(kept_weight(token, l))); },
+           b, logits, sum, kept);
 }
 
 template <typename L>
 int launch(const SampleParams& p, long long rows, int ranks, cudaStream_t stream) {
-  // Head elements ahead of the first aligned one shift the slice by up to a vector.
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (static_cast<size_t>(p.slice) + 8) * 4;
+  const size_t smem = kSharedBytes + static_cast<size_t>(p.slice) * sizeof(L);  // slice: whole vectors
   const cudaError_t err = cudaFuncSetAttribute(
       sample_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (err != cudaSuccess) return cuda_status(err, "sample_kernel shared memory");
