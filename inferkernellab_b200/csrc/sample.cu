@@ -54,6 +54,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kList = 1024;      // tokens that are sorted
+constexpr int kCounted = 256;    // list entries up to which counting beats sorting
 constexpr int kFewTokens = 512;  // top_k up to which the threads' largest tokens bound the list
 // Bins of the threads' largest tokens: 11 per unit of (m - l) / T, so that 255 of
 // them span the weights above 2^-32; the last one holds everything below.
@@ -61,9 +62,9 @@ constexpr int kCoarse = 256;
 constexpr float kCoarsePerUnit = 11.f;
 // Bins of the exact search.
 constexpr int kBins = 1024;
-constexpr int kFirstShift = 20;                          // bits below an eighth of an octave
-constexpr uint32_t kFirstBase = (127u - 31u) << 3;       // key >> 20 of w = 2^-31
-constexpr int kFirstBins = (127 << 3) - kFirstBase + 1;  // 249: the last one holds w = 1
+constexpr int kFirstShift = 18;                          // bits below 1/32 octave
+constexpr uint32_t kFirstBase = (127u - 31u) << 5;       // key >> 18 of w = 2^-31
+constexpr int kFirstBins = (127 << 5) - kFirstBase + 1;  // 993: the last one holds w = 1
 constexpr int kMaxSlice = 46 * 1024;                     // tokens of a CTA
 constexpr float kLargest = 3.402823466e38f, kSmallest = 1.175494351e-38f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -94,12 +95,15 @@ struct Cut {  // kept: key > cut.key, or key == cut.key and index <= cut.index
 };
 
 struct Shared {
-  u64 list[kList];  // rank 0: gathered tokens, key << 32 | ~index
-  // The threads' largest tokens: count, and mass in units of 2^-22.
-  uint32_t coarse_count[kCoarse], coarse_mass[kCoarse];
+  // Rank 0: gathered tokens, key << 32 | ~index, and their logits.  A CTA of the
+  // cluster has kList / ranks places of its own.
+  u64 list[kList];
+  float list_logit[kList];
   // The exact search: a bin's mass is two 32-bit sums (low and high 16 bits; a CTA
   // holds at most 2^16 tokens), since 64-bit shared-memory atomics are loops.
   uint32_t count[kBins], low[kBins], high[kBins];
+  // The threads' largest tokens: count, and mass in units of 2^-22.
+  uint32_t coarse_count[kCoarse], coarse_mass[kCoarse];
   // Written by every CTA of the cluster, read here after the next cluster barrier.
   float max_of[kMaxCluster];
   double sum_of[kMaxCluster];
@@ -107,7 +111,7 @@ struct Shared {
   u64 warp_mass[kMaxCluster * kWarps];
   float warp_sum[kMaxCluster * kWarps];
   int warp_ties[kMaxCluster * kWarps];
-  int listed[3];  // rank 0: list entries taken (first gathering, then one per search)
+  int listed[2];  // rank 0: list entries taken, by search
   Cut cut;
   // Of this CTA alone.
   int local_first, local_listed;
@@ -178,6 +182,12 @@ __device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
 // Inclusive prefix over the lanes of a warp.
@@ -290,18 +300,15 @@ class Row {
       }
     }
     m = thread_max;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = warp_max(m);
     if (lane == 0) s.red_f[warp] = m;
     __syncthreads();
-    if (tid < ranks) {
-      m = s.red_f[0];
-      for (int i = 1; i < kWarps; ++i) m = fmaxf(m, s.red_f[i]);
-      at(tid)->max_of[rank] = m;
+    if (warp == 0) {
+      m = warp_max(s.red_f[lane % kWarps]);
+      if (lane < ranks) at(lane)->max_of[rank] = m;
     }
     cluster.sync();
-    m = s.max_of[0];
-    for (int r = 1; r < ranks; ++r) m = fmaxf(m, s.max_of[r]);
+    m = warp_max(s.max_of[min(lane, ranks - 1)]);
   }
 
   __device__ float argument(float l) const {  // of the exponential
@@ -357,14 +364,22 @@ class Row {
     float sum = 0.f;
     u64 mass = 0;
     int pass = 0;
-    each([&](int, float l) {
-      const float w = weight(l);
-      sum += w;
-      if (w >= min_p) {
+    if (m != INFINITY && min_p == 0.f) {  // the usual case, without the tests
+      each([&](int, float l) {
+        const float w = expf(__fmul_rn(__fsub_rn(l, m), inv));
+        sum += w;
         mass += mass_of(w);
-        ++pass;
-      }
-    });
+      });
+    } else {
+      each([&](int, float l) {
+        const float w = weight(l);
+        sum += w;
+        if (w >= min_p) {
+          mass += mass_of(w);
+          ++pass;
+        }
+      });
+    }
     push_sum(sum);
     mass = warp_sum(mass);
     pass = warp_sum(pass);
@@ -404,15 +419,18 @@ class Row {
   // The first coarse bin at which the threads' largest tokens of the row reach
   // `target`, or -1.
   __device__ int coarse_bound(Measure measure, u64 target) {
-    uint32_t c = 0;
-    if (tid < kCoarse)
-      for (int r = 0; r < ranks; ++r) {
-        const Shared* o = at(r);
-        c += measure == kCount ? o->coarse_count[tid] : o->coarse_mass[tid];
-        // 8 CTAs x 512 threads x 2^22: 33 bits; cap what only has to reach target
-        if (c > 0x7fffffffu) c = 0x7fffffffu;
+    u64 c = 0;  // 8 CTAs x 512 threads x 2^22: 35 bits
+    if (tid < kCoarse) {
+      uint32_t part[kMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {  // every remote load in flight at once
+        const Shared* o = at(min(r, ranks - 1));
+        part[r] = measure == kCount ? o->coarse_count[tid] : o->coarse_mass[tid];
       }
-    u64 sum = warp_prefix(static_cast<u64>(c), lane);
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) c += r < ranks ? part[r] : 0;
+    }
+    u64 sum = warp_prefix(c, lane);
     if (lane == 31) s.scan_mass[warp] = sum;
     if (tid == 0) s.found = -1;
     __syncthreads();
@@ -430,30 +448,57 @@ class Row {
     const float edge = (bound + 1) / kCoarsePerUnit / inv;
     const float limit =
         bound >= kCoarse - 1 ? -kLargest : m - edge * 1.0001f - (fabsf(m) + 1e-30f) * 1e-6f;
-    int mine = 0;
-    const bool any = thread_max >= limit;
-    if (any) each([&](int, float l) { mine += l >= limit; });
-    mine = warp_sum(mine);
-    if (lane == 0 && mine > 0) atomicAdd(&s.local_listed, mine);
-    __syncthreads();
-    const int total = s.local_listed;
-    if (any && total <= kList) {
+    const int places = kList / ranks;
+    if (thread_max >= limit) {
       Shared* home = at(0);
       each([&](int token, float l) {
         if (l >= limit) {
           const float w = weight(l);
           if (w >= min_p && w > 0.f) {
-            const int to = atomicAdd(&home->listed[0], 1);
-            if (to < kList) home->list[to] = entry(w, token);
+            const int to = atomicAdd(&s.local_listed, 1);
+            if (to < places) {
+              home->list[rank * places + to] = entry(w, token);
+              home->list_logit[rank * places + to] = l;
+            }
           }
         }
       });
     }
-    if (tid < ranks) at(tid)->listed_of[rank] = total;
+    __syncthreads();
+    if (tid < ranks) at(tid)->listed_of[rank] = s.local_listed;
     cluster.sync();
-    int sum = 0;
-    for (int r = 0; r < ranks; ++r) sum += s.listed_of[r];
-    return sum <= kList;
+    return warp_max(static_cast<float>(s.listed_of[min(lane, ranks - 1)])) <= places;
+  }
+
+  // Closes the gaps between the CTAs' parts of the list (rank 0); returns its length.
+  __device__ int close_list() {
+    const int places = kList / ranks;
+    u64 e[2];
+    float l[2];
+    int to[2], n = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int from = tid + i * kThreads;
+      n = 0;
+      to[i] = -1;
+      for (int r = 0; r < ranks; ++r) {
+        if (from / places == r && from % places < s.listed_of[r]) to[i] = n + from % places;
+        n += s.listed_of[r];
+      }
+      if (to[i] >= 0) {
+        e[i] = s.list[from];
+        l[i] = s.list_logit[from];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (to[i] >= 0) {
+        s.list[to[i]] = e[i];
+        s.list_logit[to[i]] = l[i];
+      }
+    __syncthreads();
+    return n;
   }
 
   __device__ static u64 entry(float w, int token) {
@@ -535,6 +580,110 @@ class Row {
     return q;
   }
 
+  template <bool kWarp, typename T>
+  __device__ T sum_over(T v, T* red) {  // of the warp, or of the block
+    v = warp_sum(v);
+    if (kWarp) return v;
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = 0;
+    for (int i = 0; i < kWarps; ++i) v += red[i];
+    return v;
+  }
+
+  // The cut and the draw among the first n list entries (rank 0), by counting for
+  // each entry what precedes it: of one warp if n <= 32, else of the block.
+  template <bool kWarp, typename F>
+  __device__ void finish(int n, int top_k, bool cut_p, bool of_list, F&& top_p_target, u64 mass,
+                         bool greedy, float u, long long b, double sum) {
+    const u64 mine = tid < n ? s.list[tid] : 0;
+    const uint32_t key = static_cast<uint32_t>(mine >> 32);
+    const uint32_t q = mass_of_key(key);
+    int rank_of = 0;
+    u64 before = 0;
+    for (int j = 0; j < n; ++j) {
+      const u64 o = s.list[j];
+      if (o > mine) {
+        ++rank_of;
+        before += mass_of_key(static_cast<uint32_t>(o >> 32));
+      }
+    }
+    bool kept = tid < n && rank_of < top_k;
+    if (cut_p) {
+      if (of_list) mass = sum_over<kWarp>(static_cast<u64>(kept ? q : 0), s.scan_mass);
+      kept = kept && before < top_p_target(mass);
+    }
+    const double kept_sum =
+        sum_over<kWarp>(static_cast<double>(kept ? __uint_as_float(key) : 0.f), s.red_d);
+    if (greedy) {  // the first largest logit, which is always kept
+      if (tid == 0) write(b, first_largest(), m, sum, kept_sum);
+      return;
+    }
+    const u64 t = draw_target(u, sum_over<kWarp>(static_cast<u64>(kept ? q : 0), s.scan_mass));
+    // Kept entries alone, then what precedes mine in order of index (~index falls).
+    if (tid < n && !kept) s.list[tid] = 0;
+    if (kWarp)
+      __syncwarp();
+    else
+      __syncthreads();
+    before = 0;
+    for (int j = 0; j < n; ++j) {
+      const u64 o = s.list[j];
+      if (static_cast<uint32_t>(o) > static_cast<uint32_t>(mine))
+        before += mass_of_key(static_cast<uint32_t>(o >> 32));
+    }
+    if (kept && before <= t && t < before + q)
+      write(b, static_cast<int>(~static_cast<uint32_t>(mine)), s.list_logit[tid], sum, kept_sum);
+  }
+
+  // The same by sorting, where counting would take longer.
+  template <typename F>
+  __device__ void finish_sorted(int n, int top_k, bool cut_p, bool of_list, F&& top_p_target,
+                                u64 mass, bool greedy, float u, long long b, const L* logits,
+                                double sum) {
+    sort_list(n);
+    int kept = min(n, top_k);
+    if (cut_p) {
+      if (of_list) mass = list_mass(kept);
+      const int pos = list_position(kept, 32, kMass, 0, top_p_target(mass), 0, nullptr);
+      kept = min(kept, pos + 1);
+    }
+    double kept_sum = 0;
+    u64 e[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = tid + i * kThreads;
+      e[i] = at < kept ? s.list[at] : 0;
+      kept_sum += __uint_as_float(static_cast<uint32_t>(e[i] >> 32));
+    }
+    kept_sum = sum_over<false>(kept_sum, s.red_d);
+    if (greedy) {
+      if (tid == 0) write(b, first_largest(), m, sum, kept_sum);
+      return;
+    }
+    const u64 total = list_mass(kept);
+    // The kept tokens by index: ~index above the key.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = tid + i * kThreads;
+      if (at < kept) s.list[at] = e[i] << 32 | e[i] >> 32;
+    }
+    __syncthreads();
+    sort_list(kept);
+    const int pos = list_position(kept, 0, kMass, 0, draw_target(u, total) + 1, 0, nullptr);
+    if (tid == 0) {
+      const int token = static_cast<int>(~static_cast<uint32_t>(s.list[pos] >> 32));
+      write(b, token, fmaxf(static_cast<float>(logits[token]), -INFINITY), sum, kept_sum);
+    }
+  }
+
+  __device__ int first_largest() const {
+    int first = p.vocab;
+    for (int r = 0; r < ranks; ++r) first = min(first, s.first_of[r]);
+    return first;
+  }
+
   // --------------------------------------------------------- exact search
   __device__ void clear_histogram() {
     for (int i = tid; i < kBins; i += kThreads) s.count[i] = s.low[i] = s.high[i] = 0;
@@ -562,14 +711,20 @@ class Row {
       uint32_t c = 0;
       u64 q = 0;
       if (bin >= (first_level ? 1 : 0)) {
-        u64 lo = 0, hi = 0;
-        for (int r = 0; r < ranks; ++r) {
-          const Shared* o = at(r);
-          c += o->count[bin];
-          lo += o->low[bin];
-          hi += o->high[bin];
+        uint32_t part[3][kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {  // every remote load in flight at once
+          const Shared* o = at(min(r, ranks - 1));
+          part[0][r] = o->count[bin];
+          part[1][r] = o->low[bin];
+          part[2][r] = o->high[bin];
         }
-        q = lo + (hi << 16);
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < ranks) {
+            c += part[0][r];
+            q += part[1][r] + (static_cast<u64>(part[2][r]) << 16);
+          }
       }
       uint32_t ci = warp_prefix(c, lane);
       u64 qi = warp_prefix(q, lane);
@@ -628,8 +783,9 @@ class Row {
     uint32_t lo = s.found_bin == 0 ? 0u : (kFirstBase + s.found_bin) << kFirstShift;
     uint32_t size = s.found_bin == 0 ? (kFirstBase + 1) << kFirstShift : 1u << kFirstShift;
     while (s.found_count > kList && size > 1) {
-      const int shift = size > (1u << kFirstShift) ? kFirstShift : (size > kBins ? 10 : 0);
-      const int bins = static_cast<int>((size + (1u << shift) - 1) >> shift);
+      int shift = 0;  // 1024 bins or fewer over [lo, lo + size)
+      while (((size - 1) >> shift) >= kBins) ++shift;
+      const int bins = static_cast<int>((size - 1) >> shift) + 1;
       const uint32_t before_count = s.before_count;
       const u64 before_mass = s.before_mass;
       clear_histogram();
@@ -665,7 +821,7 @@ class Row {
 
   // At most kList tokens with keys in [lo, lo + size): sorted by rank 0.
   __device__ void resolve_listed(Measure measure, u64 target, uint32_t lo, uint32_t size) {
-    const int slot = 1 + searches;
+    const int slot = searches;
     const u64 before_mass = s.before_mass;
     const u64 before = measure == kCount ? s.before_count : before_mass;
     Shared* home = at(0);
@@ -706,7 +862,7 @@ class Row {
       walk(before, [&](int token, float l) {
         const float w = weight(l);
         return static_cast<u64>(__float_as_uint(w) == key && w >= min_p && in_slice(token));
-      }, r - 1, [&](int token) {
+      }, r - 1, [&](int token, float) {
         Cut cut = found;
         cut.index = token;
         for (int o = 0; o < ranks; ++o) at(o)->cut = cut;
@@ -716,7 +872,7 @@ class Row {
   }
 
   // Walks this warp's run in order of index, adding value(token, logit) to
-  // `running`; done(token) is called by one lane for the first token that takes it
+  // `running`; done(token, logit) is called by one lane for the first token that takes it
   // past t.
   template <typename F, typename G>
   __device__ void walk(u64 running, F&& value, u64 t, G&& done) {
@@ -734,16 +890,18 @@ class Row {
         if (lane == __ffs(vote) - 1) {
           u64 before = with - sum;
           int token = 0;
+          float l = 0.f;
           bool open = true;
 #pragma unroll
           for (int i = 0; i < kN; ++i) {
             before += q[i];
             if (open && before > t) {
               token = origin + (v + lane) * kN + i;
+              l = raw[v + lane].get(i);
               open = false;
             }
           }
-          done(token);
+          done(token, l);
         }
         return;
       }
@@ -759,22 +917,23 @@ class Row {
     return t < total ? t : total - 1;
   }
 
-  // One thread of the cluster writes the row's results.
-  __device__ void write(long long b, int token, const L* logits, double sum, double kept) {
-    const double x = argument(fmaxf(static_cast<float>(logits[token]), -INFINITY));
+  // One thread of the cluster writes the row's results; sums are at least 1 (w of
+  // the largest), and what they are above it keeps its digits.
+  __device__ void write(long long b, int token, float l, double sum, double kept) {
+    const float x = argument(l);
     p.tokens[b] = token;
-    p.logprobs[b] = static_cast<float>(x - log(sum));
-    p.sampling_logprobs[b] = static_cast<float>(x - log(kept));
+    p.logprobs[b] = x - log1pf(static_cast<float>(sum - 1.0));
+    p.sampling_logprobs[b] = x - log1pf(static_cast<float>(kept - 1.0));
   }
 
   // The token at mass t of the row, whose warps' masses are in place.
   template <typename F>
-  __device__ void draw(float u, F&& value, long long b, const L* logits, double sum, double kept) {
+  __device__ void draw(float u, F&& value, long long b, double sum, double kept) {
     const u64 t = draw_target(u, row_mass());
     const int me = rank * kWarps + warp;
     const u64 before = mass_before(me);
     if (before <= t && t < before + s.warp_mass[me])  // warp-uniform
-      walk(before, value, t, [&](int token) { write(b, token, logits, sum, kept); });
+      walk(before, value, t, [&](int token, float l) { write(b, token, l, sum, kept); });
   }
 };
 
@@ -788,7 +947,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const long long b = blockIdx.x / row.ranks;
   if (tid < kCoarse) s.coarse_count[tid] = s.coarse_mass[tid] = 0;
   if (tid == 0) {
-    s.listed[0] = s.listed[1] = s.listed[2] = s.local_listed = 0;
+    s.listed[0] = s.listed[1] = s.local_listed = 0;
     s.local_first = p.vocab;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -829,15 +988,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   row.push_block_sums(exact, greedy);
   cluster.sync();
   const double sum = row.row_sum();
-  int first = p.vocab;
-  if (greedy)
-    for (int r = 0; r < row.ranks; ++r) first = min(first, s.first_of[r]);
   if (!filtered) {
     if (!greedy)
-      row.draw(u, [&](int, float l) { return static_cast<u64>(mass_of(row.weight(l))); }, b, logits,
-               sum, sum);
+      row.draw(u, [&](int, float l) { return static_cast<u64>(mass_of(row.weight(l))); }, b, sum,
+               sum);
     else if (rank == 0 && tid == 0)
-      row.write(b, first, logits, sum, sum);
+      row.write(b, row.first_largest(), row.m, sum, sum);
     return;
   }
 
@@ -859,47 +1015,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     if (bound >= 0 && row.gather(bound)) {  // cluster-uniform
       if (rank != 0) return;
-      const int n = s.listed[0];
-      int kept = n;
-      if (cut_k || cut_p) {
-        row.sort_list(n);
-        if (cut_k) kept = min(n, top_k);
-        if (cut_p) {
-          const u64 mass = few ? row.list_mass(kept) : row.row_mass();
-          const int pos = row.list_position(kept, 32, kMass, 0, top_p_target(mass), 0, nullptr);
-          kept = min(kept, pos + 1);
-        }
+      const int n = row.close_list();
+      const u64 mass = few || !cut_p ? 0 : row.row_mass();
+      if (n <= 32) {
+        if (warp == 0)
+          row.template finish<true>(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy,
+                                    u, b, sum);
+      } else if (n <= kCounted) {
+        row.template finish<false>(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy, u,
+                                   b, sum);
+      } else {
+        row.finish_sorted(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy, u, b,
+                          logits, sum);
       }
-      // The kept tokens by index, and their sum.
-      double kept_sum = 0;
-      u64 e[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = tid + i * kThreads;
-        e[i] = at < kept ? s.list[at] : 0;
-        kept_sum += __uint_as_float(static_cast<uint32_t>(e[i] >> 32));
-      }
-      const u64 total = row.list_mass(kept);
-      kept_sum = warp_sum(kept_sum);
-      if (lane == 0) s.red_d[warp] = kept_sum;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = tid + i * kThreads;
-        if (at < kept) s.list[at] = e[i] << 32 | e[i] >> 32;  // ~index above the key
-      }
-      __syncthreads();
-      kept_sum = 0;
-      for (int i = 0; i < kWarps; ++i) kept_sum += s.red_d[i];
-      if (greedy) {
-        if (tid == 0) row.write(b, first, logits, sum, kept_sum);
-        return;
-      }
-      row.sort_list(kept);
-      const int pos = row.list_position(kept, 0, kMass, 0, Row<L>::draw_target(u, total) + 1, 0,
-                                        nullptr);
-      if (tid == 0)
-        row.write(b, static_cast<int>(~static_cast<uint32_t>(s.list[pos] >> 32)), logits, sum,
-                  kept_sum);
       return;
     }
   }
@@ -946,11 +1074,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   for (int i = lane; i < row.ranks * kWarps; i += 32) kept += s.warp_sum[i];
   kept = warp_sum(kept);
   if (greedy) {
-    if (rank == 0 && tid == 0) row.write(b, first, logits, sum, kept);
+    if (rank == 0 && tid == 0) row.write(b, row.first_largest(), row.m, sum, kept);
     return;
   }
   row.draw(u, [&](int token, float l) { return static_cast<u64>(mass_of(kept_weight(token, l))); },
-           b, logits, sum, kept);
+           b, sum, kept);
 }
 
 template <typename L>
