@@ -29,6 +29,8 @@ namespace b200 {
 
 namespace {
 
+constexpr int kRowsAtOnce = 4;
+
 struct QkNormParams {
   const uint8_t* q;
   const uint8_t* k;
@@ -50,49 +52,123 @@ struct QkNormParams {
 
 // 8 x 16-bit elements = one 16-byte access.
 struct alignas(16) Vec8 {
-  uint16_t h[8];
+  uint32_t w[4];
+};
+
+// The two values of a packed pair.
+template <typename E>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<Half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<BF16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+template <typename E>
+__device__ __forceinline__ void widen(const Vec8& v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = unpack2<E>(v.w[i]);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+}
+template <typename E>
+__device__ __forceinline__ Vec8 narrow(const float (&f)[8]) {
+  Vec8 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.w[i] = pack2<E>(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+
+// Row `row` of token t: q heads, then k heads, then v heads.
+template <typename T>
+__device__ __forceinline__ const T* source_row(const QkNormParams& p, long long t, int row) {
+  if (row < p.num_q_heads) return reinterpret_cast<const T*>(p.q) + t * p.q_st + row * p.q_sh;
+  const int h = row - p.num_q_heads;
+  if (h < p.num_kv_heads) return reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh;
+  return reinterpret_cast<const T*>(p.v) + t * p.v_st + (h - p.num_kv_heads) * p.v_sh;
+}
+template <typename T>
+__device__ __forceinline__ T* target_row(const QkNormParams& p, long long t, int row,
+                                         long long slot) {
+  if (row < p.num_q_heads) return reinterpret_cast<T*>(p.q_out) + t * p.qo_st + row * p.qo_sh;
+  const int h = row - p.num_q_heads;
+  const bool is_k = h < p.num_kv_heads;
+  return reinterpret_cast<T*>(is_k ? p.k_cache : p.v_cache) +
+         ((p.layer_slot_base + slot) * p.num_kv_heads + (is_k ? h : h - p.num_kv_heads)) *
+             p.head_dim;
+}
+
+// What a lane multiplies its 8 pairs (a, b) with, apart from the row's 1 / rms:
+//   lo = a * ac + b * bs,   hi = b * bc + a * as
+// the weight times cos or sin (1 and 0 where nothing is rotated).
+struct Factors {
+  float ac[8], bs[8], bc[8], as[8];
 };
 
 template <typename E>
-__device__ __forceinline__ float lane_f(const Vec8& v, int i) {
-  typename E::T t;
-  memcpy(&t, &v.h[i], 2);
-  return to_float<E>(t);
-}
-
-template <typename E>
-__device__ __forceinline__ void lane_set(Vec8& v, int i, float x) {
-  typename E::T t = from_float<E>(x);
-  memcpy(&v.h[i], &t, 2);
-}
-
-// Source and destination of row `row` of token t: q heads, then k heads, then v
-// heads.  kind 0: q, 1: k, 2: v.
-template <typename T>
-__device__ __forceinline__ int row_pointers(const QkNormParams& p, long long t, int row,
-                                            long long slot, const T** src, T** dst) {
-  const int kv = p.num_kv_heads;
-  if (row < p.num_q_heads) {
-    *src = reinterpret_cast<const T*>(p.q) + t * p.q_st + row * p.q_sh;
-    *dst = reinterpret_cast<T*>(p.q_out) + t * p.qo_st + row * p.qo_sh;
-    return 0;
+__device__ __forceinline__ Factors factors(const void* weight, int lo, int hi, bool rotated,
+                                           const Vec8& c1, const Vec8& c2, const Vec8& s1,
+                                           const Vec8& s2) {
+  using T = typename E::T;
+  Factors f;
+  float w1[8], w2[8], c[8], s[8];
+  widen<E>(*reinterpret_cast<const Vec8*>(reinterpret_cast<const T*>(weight) + lo), w1);
+  widen<E>(*reinterpret_cast<const Vec8*>(reinterpret_cast<const T*>(weight) + hi), w2);
+  widen<E>(c1, c);
+  widen<E>(s1, s);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f.ac[j] = rotated ? w1[j] * c[j] : w1[j];
+    f.bs[j] = rotated ? -w2[j] * s[j] : 0.f;
   }
-  const bool is_k = row < p.num_q_heads + kv;
-  const int h = row - p.num_q_heads - (is_k ? 0 : kv);
-  *src = is_k ? reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh
-              : reinterpret_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh;
-  *dst = reinterpret_cast<T*>(is_k ? p.k_cache : p.v_cache) +
-         ((p.layer_slot_base + slot) * kv + h) * p.head_dim;
-  return is_k ? 1 : 2;
+  widen<E>(c2, c);
+  widen<E>(s2, s);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f.bc[j] = rotated ? w2[j] * c[j] : w2[j];
+    f.as[j] = rotated ? w1[j] * s[j] : 0.f;
+  }
+  return f;
 }
 
-// One CTA per token; LANES = D / 16 lanes per row, blockDim a multiple of 32.
+// Normalises and turns one row, whose LANES lanes all call it.
 template <typename E, int LANES>
+__device__ __forceinline__ void norm_turn(Vec8& x1, Vec8& x2, const Factors& f, float inv_dim,
+                                          float eps) {
+  float a[8], b[8];
+  widen<E>(x1, a);
+  widen<E>(x2, b);
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss = fmaf(a[j], a[j], fmaf(b[j], b[j], ss));
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float inv = rsqrtf(ss * inv_dim + eps);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = a[j] * inv, y = b[j] * inv;
+    a[j] = fmaf(x, f.ac[j], y * f.bs[j]);
+    b[j] = fmaf(y, f.bc[j], x * f.as[j]);
+  }
+  x1 = narrow<E>(a);
+  x2 = narrow<E>(b);
+}
+
+// One CTA per token; LANES = D / 16 lanes per row, the rows of the CTA's groups of
+// lanes G apart.  A lane's factors are the same for all heads of q (of k), so they
+// are formed once for the ROWS q rows that it takes at a time (all of their loads
+// in flight together) and once more for its k row, which it reads with the v row.
+template <typename E, int LANES, int ROWS>
 __global__ void __launch_bounds__(512) qk_norm_vec_kernel(const QkNormParams p) {
   using T = typename E::T;
   const long long t = blockIdx.x;
-  const int rows = p.num_q_heads + 2 * p.num_kv_heads;
   const int part = threadIdx.x % LANES;
+  const int group = threadIdx.x / LANES, groups = blockDim.x / LANES;
   const int rot_half = p.rotary_dim / 2;
   // The 8 pairs of this lane: rotated ones first, then the dimensions past R
   // taken as pairs half of their count apart.
@@ -100,8 +176,10 @@ __global__ void __launch_bounds__(512) qk_norm_vec_kernel(const QkNormParams p) 
   const int past = part * 8 - rot_half;
   const int lo = rotated ? part * 8 : p.rotary_dim + past;
   const int hi = rotated ? lo + rot_half : lo + (p.head_dim - p.rotary_dim) / 2;
+  const float inv_dim = 1.f / static_cast<float>(p.head_dim);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  Vec8 c1, c2, s1, s2;
+  const long long slot = load_index(p.slots, t, p.slots64);
+  Vec8 c1 = {}, c2 = {}, s1 = {}, s2 = {};
   if (rotated) {
     const T* c = reinterpret_cast<const T*>(p.cos) + t * p.cos_st;
     const T* s = reinterpret_cast<const T*>(p.sin) + t * p.sin_st;
@@ -110,49 +188,72 @@ __global__ void __launch_bounds__(512) qk_norm_vec_kernel(const QkNormParams p) 
     s1 = *reinterpret_cast<const Vec8*>(s + lo);
     s2 = *reinterpret_cast<const Vec8*>(s + hi);
   }
-  const long long slot = load_index(p.slots, t, p.slots64);
-  const bool slot_ok = slot >= 0 && slot < p.num_slots;
-  if (slot >= p.num_slots && threadIdx.x == 0 && p.err) atomicOr(p.err, kErrBadSlot);
-  const int per_pass = blockDim.x / LANES;
-  const int lane_row = threadIdx.x / LANES;
-  // Whole warps walk the rows together: the shuffles below need every lane.
-  for (int base = 0; base < rows; base += per_pass) {
-    if (base + (threadIdx.x & ~31) / LANES >= rows) break;  // warp-uniform
-    const int row = base + lane_row;
-    const bool live = row < rows && (row < p.num_q_heads || slot_ok);
-    const T* src = nullptr;
-    T* dst = nullptr;
-    int kind = 2;
-    Vec8 x1 = {}, x2 = {};
-    if (live) {
-      kind = row_pointers<T>(p, t, row, slot, &src, &dst);
-      x1 = *reinterpret_cast<const Vec8*>(src + lo);
-      x2 = *reinterpret_cast<const Vec8*>(src + hi);
-    }
-    float ss = 0.f;
+  // k and v rows start at the group after the last q row's, so that a CTA with a
+  // group per row works on all of them at once.
+  const int kv0 = (group + groups - p.num_q_heads % groups) % groups;
+  Vec8 k1 = {}, k2 = {}, v1 = {}, v2 = {};
+  if (kv0 < p.num_kv_heads) {
+    const T* k = reinterpret_cast<const T*>(p.k) + t * p.k_st + kv0 * p.k_sh;
+    const T* v = reinterpret_cast<const T*>(p.v) + t * p.v_st + kv0 * p.v_sh;
+    k1 = *reinterpret_cast<const Vec8*>(k + lo);
+    k2 = *reinterpret_cast<const Vec8*>(k + hi);
+    v1 = *reinterpret_cast<const Vec8*>(v + lo);
+    v2 = *reinterpret_cast<const Vec8*>(v + hi);
+  }
+  // Whole warps walk the rows together: the sums need every lane.
+  const int warp_group = static_cast<int>(threadIdx.x & ~31) / LANES;
+  if (warp_group < p.num_q_heads) {
+    const T* q = reinterpret_cast<const T*>(p.q) + t * p.q_st;
+    T* out = reinterpret_cast<T*>(p.q_out) + t * p.qo_st;
+    for (int base = 0; base + warp_group < p.num_q_heads; base += groups * ROWS) {
+      Vec8 x1[ROWS], x2[ROWS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = lane_f<E>(x1, j), b = lane_f<E>(x2, j);
-      ss = fmaf(a, a, fmaf(b, b, ss));
-    }
+      for (int i = 0; i < ROWS; ++i) {
+        const int row = base + i * groups + group;
+        x1[i] = x2[i] = Vec8{};
+        if (row < p.num_q_heads) {
+          x1[i] = *reinterpret_cast<const Vec8*>(q + row * p.q_sh + lo);
+          x2[i] = *reinterpret_cast<const Vec8*>(q + row * p.q_sh + hi);
+        }
+      }
+      const Factors f = factors<E>(p.q_weight, lo, hi, rotated, c1, c2, s1, s2);
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live) continue;
-    if (kind != 2) {
-      const float inv = rsqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
-      const T* w = reinterpret_cast<const T*>(kind == 0 ? p.q_weight : p.k_weight);
-      const Vec8 w1 = *reinterpret_cast<const Vec8*>(w + lo);
-      const Vec8 w2 = *reinterpret_cast<const Vec8*>(w + hi);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = lane_f<E>(x1, j) * inv * lane_f<E>(w1, j);
-        const float b = lane_f<E>(x2, j) * inv * lane_f<E>(w2, j);
-        lane_set<E>(x1, j, rotated ? a * lane_f<E>(c1, j) - b * lane_f<E>(s1, j) : a);
-        lane_set<E>(x2, j, rotated ? b * lane_f<E>(c2, j) + a * lane_f<E>(s2, j) : b);
+      for (int i = 0; i < ROWS; ++i) {
+        const int row = base + i * groups + group;
+        norm_turn<E, LANES>(x1[i], x2[i], f, inv_dim, p.eps);
+        if (row < p.num_q_heads) {
+          *reinterpret_cast<Vec8*>(out + row * p.qo_sh + lo) = x1[i];
+          *reinterpret_cast<Vec8*>(out + row * p.qo_sh + hi) = x2[i];
+        }
       }
     }
-    *reinterpret_cast<Vec8*>(dst + lo) = x1;
-    *reinterpret_cast<Vec8*>(dst + hi) = x2;
+  }
+  if (slot < 0 || slot >= p.num_slots) {  // CTA-uniform: nothing to append
+    if (slot >= p.num_slots && threadIdx.x == 0 && p.err) atomicOr(p.err, kErrBadSlot);
+    return;
+  }
+  if (!__any_sync(0xffffffffu, kv0 < p.num_kv_heads)) return;
+  const Factors f = factors<E>(p.k_weight, lo, hi, rotated, c1, c2, s1, s2);
+  const long long at = (p.layer_slot_base + slot) * p.num_kv_heads;
+  for (int h = kv0; __any_sync(0xffffffffu, h < p.num_kv_heads); h += groups) {
+    const bool live = h < p.num_kv_heads;
+    if (h != kv0 && live) {
+      const T* k = reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh;
+      const T* v = reinterpret_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh;
+      k1 = *reinterpret_cast<const Vec8*>(k + lo);
+      k2 = *reinterpret_cast<const Vec8*>(k + hi);
+      v1 = *reinterpret_cast<const Vec8*>(v + lo);
+      v2 = *reinterpret_cast<const Vec8*>(v + hi);
+    }
+    norm_turn<E, LANES>(k1, k2, f, inv_dim, p.eps);
+    if (live) {
+      T* k = reinterpret_cast<T*>(p.k_cache) + (at + h) * p.head_dim;
+      T* v = reinterpret_cast<T*>(p.v_cache) + (at + h) * p.head_dim;
+      *reinterpret_cast<Vec8*>(k + lo) = k1;
+      *reinterpret_cast<Vec8*>(k + hi) = k2;
+      *reinterpret_cast<Vec8*>(v + lo) = v1;
+      *reinterpret_cast<Vec8*>(v + hi) = v2;
+    }
   }
 }
 
@@ -172,9 +273,9 @@ __global__ void __launch_bounds__(1024) qk_norm_any_kernel(const QkNormParams p)
   if (slot >= p.num_slots && threadIdx.x == 0 && p.err) atomicOr(p.err, kErrBadSlot);
   for (int row = threadIdx.x >> 5; row < rows; row += blockDim.x >> 5) {
     if (row >= p.num_q_heads && !slot_ok) continue;
-    const T* src;
-    T* dst;
-    const int kind = row_pointers<T>(p, t, row, slot, &src, &dst);
+    const T* src = source_row<T>(p, t, row);
+    T* dst = target_row<T>(p, t, row, slot);
+    const int kind = row < p.num_q_heads ? 0 : row < p.num_q_heads + p.num_kv_heads ? 1 : 2;
     if (kind == 2) {
       for (int i = lane; i < p.head_dim; i += 32) dst[i] = src[i];
       continue;
@@ -201,23 +302,34 @@ __global__ void __launch_bounds__(1024) qk_norm_any_kernel(const QkNormParams p)
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename E>
-cudaError_t launch(const QkNormParams& p, long long tokens, bool vec, cudaStream_t stream) {
-  const long long rows = p.num_q_heads + 2LL * p.num_kv_heads;
-  const int lanes = vec ? p.head_dim / 16 : 32;
-  // Every row of a token at once where the threads allow.
-  const dim3 block(static_cast<unsigned>(std::min<long long>(vec ? 512 : 1024, (rows * lanes + 31) / 32 * 32)));
-  const dim3 grid(static_cast<unsigned>(tokens));
-  void (*kern)(QkNormParams) = qk_norm_any_kernel<E>;
-  if (vec) {
-    switch (lanes) {
-      case 1: kern = qk_norm_vec_kernel<E, 1>; break;
-      case 2: kern = qk_norm_vec_kernel<E, 2>; break;
-      case 4: kern = qk_norm_vec_kernel<E, 4>; break;
-      case 8: kern = qk_norm_vec_kernel<E, 8>; break;
-      default: kern = qk_norm_vec_kernel<E, 16>; break;
-    }
+template <typename E, int ROWS>
+void (*vec_kernel(int lanes))(QkNormParams) {
+  switch (lanes) {
+    case 1: return qk_norm_vec_kernel<E, 1, ROWS>;
+    case 2: return qk_norm_vec_kernel<E, 2, ROWS>;
+    case 4: return qk_norm_vec_kernel<E, 4, ROWS>;
+    case 8: return qk_norm_vec_kernel<E, 8, ROWS>;
+    default: return qk_norm_vec_kernel<E, 16, ROWS>;
   }
+}
+
+template <typename E>
+cudaError_t launch(const QkNormParams& p, long long tokens, bool vec, int sms,
+                   cudaStream_t stream) {
+  const int lanes = vec ? p.head_dim / 16 : 32;
+  // More than a token per SM: ROWS q rows per thread, for the bytes in flight and
+  // the factors formed once.  Fewer: a group of lanes per row, for the shortest
+  // way through.
+  const bool many = vec && tokens > sms;
+  const long long groups = many  ? ceil_div64(p.num_q_heads, kRowsAtOnce)
+                           : vec ? p.num_q_heads + p.num_kv_heads
+                                 : p.num_q_heads + 2LL * p.num_kv_heads;
+  const dim3 block(static_cast<unsigned>(
+      std::min<long long>(vec ? 512 : 1024, (groups * lanes + 31) / 32 * 32)));
+  const dim3 grid(static_cast<unsigned>(tokens));
+  void (*kern)(QkNormParams) = !vec ? qk_norm_any_kernel<E>
+                               : many   ? vec_kernel<E, kRowsAtOnce>(lanes)
+                                      : vec_kernel<E, 1>(lanes);
   return launch_dependent(kern, grid, block, 0, stream, p);
 }
 
@@ -292,8 +404,12 @@ int launch_qk_norm_rope_append(const b200_cache_desc* c, const b200_qk_norm_args
                    aligned16(q_weight) && aligned16(k_weight) && aligned16(cos) &&
                    aligned16(sin) && aligned16(query_out) && aligned16(c->k_cache) &&
                    aligned16(c->v_cache);
-  return cuda_status(c->dtype == B200_BF16 ? launch<BF16>(p, a->num_tokens, vec, stream)
-                                           : launch<Half>(p, a->num_tokens, vec, stream),
+  DeviceInfo info;
+  const int rc = current_device_info(&info);
+  if (rc != B200_OK) return rc;
+  return cuda_status(c->dtype == B200_BF16
+                         ? launch<BF16>(p, a->num_tokens, vec, info.num_sms, stream)
+                         : launch<Half>(p, a->num_tokens, vec, info.num_sms, stream),
                      "qk_norm kernel launch");
 }
 
