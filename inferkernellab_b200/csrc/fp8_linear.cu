@@ -60,6 +60,14 @@ struct Shape {
   static constexpr int kEpi = TOKENS > 128 ? 8 : 4;  // epilogue warps
   static constexpr int kThreads = (kEpi + 4) * 32;
   static constexpr int kCols = TOKENS / (kEpi / 4);  // token columns of an epilogue thread
+  static constexpr int kStep = kCols < 32 ? kCols : 32;  // columns of one TMEM load
+  // 256 tokens: 128 sums and 64 loaded values per epilogue thread are more than the
+  // 168 registers of 384 threads, so that the other four warps give some of theirs.
+  static constexpr bool kSplitRegisters = TOKENS > 128;
+  static constexpr int kEpiRegisters = 224, kOtherRegisters = 56, kLaunchRegisters = 168;
+  static_assert(kEpi * kEpiRegisters + 4 * kOtherRegisters <= (kEpi + 4) * kLaunchRegisters ||
+                    !kSplitRegisters,
+                "what the epilogue takes is what the other warps give");
   static constexpr int kStageBytes = kRows * kBlock + TOKENS * kBlock;
   // Up to 64 tokens a CTA takes under half an SM, so that two share it: the
   // product is then bound by the weight's bytes, and 296 CTAs spread them
@@ -105,6 +113,13 @@ __device__ __forceinline__ float2 unpack_f32x2(u64 v) {
   float2 f;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
   return f;
+}
+
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[32]) {
+  tc::ld32(taddr, v);
+}
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[16]) {
+  tc::ld16(taddr, v);
 }
 
 template <typename E, int TOKENS>
@@ -164,104 +179,106 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
   const uint32_t tmem = *tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  if (warp == S::kEpi) {
-    // ------------------------------ producer ------------------------------
-    if (lane == 0) {
-      tma_prefetch_desc(&wmap);
-      tma_prefetch_desc(&xmap);
-      int it = 0;
-      bool ok = true;
-      for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-        const int n0 = static_cast<int>(tile / p.token_tiles) * kRows;
-        const int m0 = static_cast<int>(tile % p.token_tiles) * TOKENS;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % kStages;
-          ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
-                                 kErrWaitEmpty);
-          if (!ok) break;
-          uint8_t* dst = stages + s * S::kStageBytes;
-          mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-          tma_load_2d(dst, &wmap, &full[s], kb * kBlock, n0);
-          tma_load_2d(dst + kRows * kBlock, &xmap, &full[s], kb * kBlock, m0);
-        }
-      }
-      drain_stages<kStages>(full, it, p.err);
-    }
-  } else if (warp == S::kEpi + 1) {
-    // ------------------------------ MMA issuer ----------------------------
-    if (lane == 0) {
-      const uint32_t idesc = tc::idesc_e4m3(kRows, TOKENS);
-      const uint32_t st0 = smem_u32(stages);
-      int it = 0;
-      bool ok = true;
-      for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % kStages, b = it % kBuffers;
-          ok = mbar_wait_bounded(&acc_empty[b], ((it / kBuffers) & 1) ^ 1, abort_flag, p.err,
-                                 kErrWaitEmpty) &&
-               mbar_wait_bounded(&full[s], (it / kStages) & 1, abort_flag, p.err, kErrWaitFull);
-          if (!ok) break;
-          tc::fence_after_sync();
-          const uint32_t w = st0 + s * S::kStageBytes;
-          const uint32_t x = w + kRows * kBlock;
-#pragma unroll
-          for (int k = 0; k < kBlock / 32; ++k)
-            tc::mma_e4m3(tmem + b * S::kBufferCols, tc::sdesc_sw128(w + k * 32, 16, 1024),
-                         tc::sdesc_sw128(x + k * 32, 16, 1024), idesc, k > 0);
-          tc::commit(&empty[s]);
-          tc::commit(&acc_full[b]);
-        }
-      }
-      // Every MMA this thread issued has finished before TMEM can be freed.
-      tc::commit(mma_idle);
-      mbar_wait_bounded(mma_idle, 0, abort_flag, p.err, kErrDrain);
-    }
-  } else if (warp == S::kEpi + 2) {
-    // ---------------------------- scale products --------------------------
-    // kAhead blocks at a time, so that their loads are in flight together.
-    constexpr int kAhead = 4;
-    constexpr int kPer = (TOKENS + 31) / 32;
-    int it = 0;
-    bool ok = true;
-    for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-      const long long m0 = tile % p.token_tiles * TOKENS;
-      const float* sw = p.w_scales + tile / p.token_tiles * p.ws_row;
-      for (int kb = kb0; kb < kb1 && ok; kb += kAhead) {
-        float v[kAhead][kPer];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          if (kb + a >= kb1) break;
-          const float ws = sw[(kb + a) * p.ws_block];
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const long long m = m0 + i * 32 + lane;
-            v[a][i] = m < p.m && i * 32 + lane < TOKENS
-                          ? p.x_scales[m * p.xs_row + (kb + a) * p.xs_block] * ws
-                          : 0.f;
-          }
-        }
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          if (kb + a >= kb1) break;
-          const int r = it % kScaleRing;
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sc_empty[r], ((it / kScaleRing) & 1) ^ 1,
-                                                         abort_flag, p.err, kErrWaitEmpty));
-          if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i)
-            if (i * 32 + lane < TOKENS) scales[r * TOKENS + i * 32 + lane] = v[a][i];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sc_full[r]);
-          ++it;
-        }
-      }
-    }
-  }
   bool ok = true;
   const int row = (warp & 3) * 32 + lane;  // of the tile; TMEM lane
   const int col0 = (warp >> 2) * S::kCols;
-  if (warp < S::kEpi) {
+  if (warp >= S::kEpi) {
+    if (S::kSplitRegisters)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegisters));
+    if (warp == S::kEpi) {
+      // ------------------------------ producer ------------------------------
+      if (lane == 0) {
+        tma_prefetch_desc(&wmap);
+        tma_prefetch_desc(&xmap);
+        int it = 0;
+        for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+          const int n0 = static_cast<int>(tile / p.token_tiles) * kRows;
+          const int m0 = static_cast<int>(tile % p.token_tiles) * TOKENS;
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % kStages;
+            ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
+                                   kErrWaitEmpty);
+            if (!ok) break;
+            uint8_t* dst = stages + s * S::kStageBytes;
+            mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+            tma_load_2d(dst, &wmap, &full[s], kb * kBlock, n0);
+            tma_load_2d(dst + kRows * kBlock, &xmap, &full[s], kb * kBlock, m0);
+          }
+        }
+        drain_stages<kStages>(full, it, p.err);
+      }
+    } else if (warp == S::kEpi + 1) {
+      // ------------------------------ MMA issuer ----------------------------
+      if (lane == 0) {
+        const uint32_t idesc = tc::idesc_e4m3(kRows, TOKENS);
+        const uint32_t st0 = smem_u32(stages);
+        int it = 0;
+        for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % kStages, b = it % kBuffers;
+            ok = mbar_wait_bounded(&acc_empty[b], ((it / kBuffers) & 1) ^ 1, abort_flag, p.err,
+                                   kErrWaitEmpty) &&
+                 mbar_wait_bounded(&full[s], (it / kStages) & 1, abort_flag, p.err, kErrWaitFull);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint32_t w = st0 + s * S::kStageBytes;
+            const uint32_t x = w + kRows * kBlock;
+#pragma unroll
+            for (int k = 0; k < kBlock / 32; ++k)
+              tc::mma_e4m3(tmem + b * S::kBufferCols, tc::sdesc_sw128(w + k * 32, 16, 1024),
+                           tc::sdesc_sw128(x + k * 32, 16, 1024), idesc, k > 0);
+            tc::commit(&empty[s]);
+            tc::commit(&acc_full[b]);
+          }
+        }
+        // Every MMA this thread issued has finished before TMEM can be freed.
+        tc::commit(mma_idle);
+        mbar_wait_bounded(mma_idle, 0, abort_flag, p.err, kErrDrain);
+      }
+    } else if (warp == S::kEpi + 2) {
+      // ---------------------------- scale products --------------------------
+      // kAhead blocks at a time, so that their loads are in flight together.
+      constexpr int kAhead = TOKENS > 128 ? 2 : 4;
+      constexpr int kPer = (TOKENS + 31) / 32;
+      int it = 0;
+      for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+        const long long m0 = tile % p.token_tiles * TOKENS;
+        const float* sw = p.w_scales + tile / p.token_tiles * p.ws_row;
+        for (int kb = kb0; kb < kb1 && ok; kb += kAhead) {
+          float v[kAhead][kPer];
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            if (kb + a >= kb1) break;
+            const float ws = sw[(kb + a) * p.ws_block];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const long long m = m0 + i * 32 + lane;
+              v[a][i] = m < p.m && i * 32 + lane < TOKENS
+                            ? p.x_scales[m * p.xs_row + (kb + a) * p.xs_block] * ws
+                            : 0.f;
+            }
+          }
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            if (kb + a >= kb1) break;
+            const int r = it % kScaleRing;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sc_empty[r], ((it / kScaleRing) & 1) ^ 1,
+                                                           abort_flag, p.err, kErrWaitEmpty));
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+              if (i * 32 + lane < TOKENS) scales[r * TOKENS + i * 32 + lane] = v[a][i];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_full[r]);
+            ++it;
+          }
+        }
+      }
+    }
+  } else {
     // ------------------------------ epilogue ------------------------------
+    if (S::kSplitRegisters)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kEpiRegisters));
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + col0;
     int it = 0;
     for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
@@ -280,24 +297,30 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
         tc::fence_after_sync();
         const ulonglong2* sc =
             reinterpret_cast<const ulonglong2*>(scales + r * TOKENS + col0);
+        // The next columns are on their way while these are added.
+        constexpr int kStep = S::kStep, kSteps = S::kCols / kStep;
+        uint32_t v[2][kStep];
+        const uint32_t base = lane_base + b * S::kBufferCols;
+        load_columns(base, v[0]);
 #pragma unroll
-        for (int c = 0; c < S::kCols; c += 16) {
-          uint32_t v[16];
-          tc::ld16(lane_base + b * S::kBufferCols + c, v);
-          tc::wait_ld();
+        for (int c = 0; c < kSteps; ++c) {
+          tc::wait_ld(v[c & 1]);
+          if (c + 1 < kSteps) {
+            load_columns(base + (c + 1) * kStep, v[(c + 1) & 1]);
+          } else {  // the buffer has been read
+            tc::fence_before_sync();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const ulonglong2 s2 = sc[c / 4 + i];
-            fma2(acc[c / 2 + 2 * i], pack_f32x2(v[4 * i], v[4 * i + 1]), s2.x);
-            fma2(acc[c / 2 + 2 * i + 1], pack_f32x2(v[4 * i + 2], v[4 * i + 3]), s2.y);
+          for (int i = 0; i < kStep / 4; ++i) {
+            const ulonglong2 s2 = sc[c * (kStep / 4) + i];
+            const int a = (c * kStep) / 2 + 2 * i;
+            fma2(acc[a], pack_f32x2(v[c & 1][4 * i], v[c & 1][4 * i + 1]), s2.x);
+            fma2(acc[a + 1], pack_f32x2(v[c & 1][4 * i + 2], v[c & 1][4 * i + 3]), s2.y);
           }
         }
-        tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&acc_empty[b]);
-          mbar_arrive(&sc_empty[r]);
-        }
+        if (lane == 0) mbar_arrive(&sc_empty[r]);
       }
       if (!ok) break;
       const long long n = tile / p.token_tiles * kRows + row;
@@ -364,6 +387,14 @@ int launch(const CUtensorMap& wmap, const CUtensorMap& xmap, const LinearParams&
   const cudaError_t err =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (err != cudaSuccess) return cuda_status(err, "fp8_linear_kernel shared memory");
+  if (S::kSplitRegisters) {
+    // Taking registers that the launch did not reserve would wait for good.
+    cudaFuncAttributes fa;
+    const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return cuda_status(e, "fp8_linear_kernel attributes");
+    if (fa.numRegs != S::kLaunchRegisters)
+      return set_error(B200_ERR_UNSUPPORTED, "fp8_linear_kernel was not built for 168 registers");
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(S::kThreads);
