@@ -11,22 +11,25 @@
 // on a 128-byte swizzled row), which the epilogue warps read from TMEM, scale and
 // add to sums in registers while the tensor core fills the next buffer.
 //
-// Orientation: the weight's rows are M of the MMA (128 per tile) and the tokens
-// are N (kTokens per tile, 16 to 256), for a decode step's few tokens as for a
-// prefill.  A thread then owns one weight row and adds, per token,
-// product * (sx * sw); the scale products of a block sit in shared memory, where
-// all 32 lanes read the same four at once.
+// Orientation.  An epilogue thread owns one row of the accumulator (a TMEM lane).
+//   Many tokens: tokens are the rows (MMA M = 128) and 128 or 256 outputs the
+//   columns, so that a thread has one scale product per block and 128 outputs, and
+//   writes neighbouring outputs of its token.  (With the outputs as rows the scales
+//   differ per column; reading 256 of them from shared memory took twice the MMAs'
+//   time, since a load returns 128 bytes a clock even where all lanes read the same.)
+//   Few tokens (up to 128): outputs are the rows and the tokens the columns, 16 to
+//   128 of them, so that the weight, which is all that counts, fills the MMA's M.
 //
 //   warps 0..kEpi-1    epilogue: warp i reads lanes 32 (i % 4) .., the columns are
 //                      split over kEpi / 4 groups
-//   warp kEpi          TMA producer: weight and token tile of a block per stage
+//   warp kEpi          TMA producer: both tiles of a block per stage
 //   warp kEpi + 1      MMA issuer (one thread)
-//   warp kEpi + 2      scale products of the blocks ahead
+//   warp kEpi + 2      scales of the blocks ahead, by asynchronous copies
 //
-// Work: tiles of 128 weight rows x kTokens tokens, tokens innermost so that
-// neighbouring CTAs share weight rows in L2.  CTAs are persistent.  Where tiles
-// are fewer than SMs, a cluster of CTAs splits K and joins its sums through
-// distributed shared memory in rank order (the result does not depend on timing).
+// Work: tiles of 128 rows x COLS columns, tokens innermost so that neighbouring
+// CTAs share weight rows in L2.  CTAs are persistent.  Where tiles are fewer than
+// SMs, a cluster of CTAs splits K and joins its sums through distributed shared
+// memory in rank order (the result does not depend on timing).
 //
 // Every mbarrier wait is bounded (1 s); on a timeout the CTA raises its abort
 // flag, records the error bit, waits (bounded) for its own copies and MMAs and
@@ -50,38 +53,44 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kRows = 128;    // weight rows of a tile = MMA M
-constexpr int kBlock = 128;   // K per scale block = bytes of a swizzled row
+constexpr int kRows = 128;   // rows of a tile = MMA M
+constexpr int kBlock = 128;  // K per scale block = bytes of a swizzled row
 constexpr int kScaleRing = 8;
 constexpr int kMaxSplits = 8;
+constexpr int kPartPitch = kRows + 1;  // of the sums that a cluster joins: both ways conflict-free
 
-template <int TOKENS>
+// TOKEN_ROWS: tokens are the tile's rows and outputs its columns; else the reverse.
+template <int COLS, bool TOKEN_ROWS>
 struct Shape {
-  static constexpr int kEpi = TOKENS > 128 ? 8 : 4;  // epilogue warps
+  static constexpr int kGroups = COLS > 128 ? 2 : 1;  // of epilogue warps, by columns
+  static constexpr int kEpi = 4 * kGroups;
   static constexpr int kThreads = (kEpi + 4) * 32;
-  static constexpr int kCols = TOKENS / (kEpi / 4);  // token columns of an epilogue thread
+  static constexpr int kCols = COLS / kGroups;         // columns of an epilogue thread
   static constexpr int kStep = kCols < 32 ? kCols : 32;  // columns of one TMEM load
-  // 256 tokens: 128 sums and 64 loaded values per epilogue thread are more than the
+  // 256 columns: 128 sums and 64 loaded values per epilogue thread are more than the
   // 168 registers of 384 threads, so that the other four warps give some of theirs.
-  static constexpr bool kSplitRegisters = TOKENS > 128;
+  static constexpr bool kSplitRegisters = COLS > 128;
   static constexpr int kEpiRegisters = 224, kOtherRegisters = 56, kLaunchRegisters = 168;
   static_assert(kEpi * kEpiRegisters + 4 * kOtherRegisters <= (kEpi + 4) * kLaunchRegisters ||
                     !kSplitRegisters,
                 "what the epilogue takes is what the other warps give");
-  static constexpr int kStageBytes = kRows * kBlock + TOKENS * kBlock;
-  // Up to 64 tokens a CTA takes under half an SM, so that two share it: the
+  static constexpr int kStageBytes = (kRows + COLS) * kBlock;
+  // Up to 64 columns a CTA takes under half an SM, so that two share it: the
   // product is then bound by the weight's bytes, and 296 CTAs spread them
   // better than 148.
-  static constexpr int kCtasPerSm = TOKENS <= 64 ? 2 : 1;
-  static constexpr int kStages = TOKENS <= 32 ? 5 : TOKENS <= 64 ? 4 : TOKENS <= 128 ? 6 : 4;
-  static constexpr int kBuffers = TOKENS > 128 ? 2 : 4;  // accumulators
-  static constexpr int kBufferCols = TOKENS < 32 ? 32 : TOKENS;
+  static constexpr int kCtasPerSm = COLS <= 64 ? 2 : 1;
+  static constexpr int kStages = COLS <= 32 ? 5 : COLS <= 64 ? 4 : COLS <= 128 ? 6 : 4;
+  static constexpr int kBuffers = COLS > 128 ? 2 : 4;  // accumulators
+  static constexpr int kBufferCols = COLS < 32 ? 32 : COLS;
   static constexpr int kTmemCols = kBuffers * kBufferCols;
-  static constexpr int kScaleBytes = kScaleRing * TOKENS * 4;
+  // Scales of a block: one per token of the tile, then one per 128 outputs.
+  static constexpr int kTokens = TOKEN_ROWS ? kRows : COLS;
+  static constexpr int kScales = (kTokens + 4 + 3) / 4 * 4;
+  static constexpr int kScaleBytes = kScaleRing * kScales * 4;
   static constexpr int kBars = 2 * kStages + 2 * kBuffers + 2 * kScaleRing + 1;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleBytes + kBars * 8 + 16;
   static_assert(kTmemCols <= 512 / kCtasPerSm, "TMEM columns");
-  static_assert(kRows * TOKENS * 4 <= kStages * kStageBytes || TOKENS > 128,
+  static_assert(kPartPitch * COLS * 4 <= kStages * kStageBytes,
                 "the split sums reuse the stages");
   static_assert(kSmem <= 227 * 1024 / kCtasPerSm - 1024, "shared memory");
 };
@@ -94,15 +103,36 @@ struct LinearParams {
   uint32_t* err;
   long long m, n;
   long long xs_row, xs_block, ws_row, ws_block, out_stride;
-  int blocks;         // of K
+  int blocks;  // of K
   int token_tiles;
   long long tiles;
   int splits;
+  int wide_stores;  // 32-byte stores of a token's outputs
 };
 
 // d += a * b on two packed 32-bit values.
 __device__ __forceinline__ void fma2(u64& d, u64 a, u64 b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 4 bytes global -> shared, asynchronous.
+__device__ __forceinline__ void copy_async_4(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
+}
+// Arrive on `bar` when this thread's asynchronous copies so far have landed.
+__device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void store_32b(void* dst, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ u64 pack_f32x2(uint32_t lo, uint32_t hi) {
   u64 d;
@@ -122,11 +152,12 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[16]) 
   tc::ld16(taddr, v);
 }
 
-template <typename E, int TOKENS>
-__global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasPerSm)
+template <typename E, int COLS, bool TOKEN_ROWS>
+__global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
+                                  Shape<COLS, TOKEN_ROWS>::kCtasPerSm)
     fp8_linear_kernel(const __grid_constant__ CUtensorMap wmap,
                       const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
-  using S = Shape<TOKENS>;
+  using S = Shape<COLS, TOKEN_ROWS>;
   using T = typename E::T;
   constexpr int kStages = S::kStages, kBuffers = S::kBuffers;
   extern __shared__ uint8_t smem_raw[];
@@ -162,7 +193,7 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
       mbar_init(&acc_empty[i], S::kEpi);
     }
     for (int i = 0; i < kScaleRing; ++i) {
-      mbar_init(&sc_full[i], 1);
+      mbar_init(&sc_full[i], 32);  // every lane's copies
       mbar_init(&sc_empty[i], S::kEpi);
     }
     mbar_init(mma_idle, 1);
@@ -181,7 +212,8 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
 
   bool ok = true;
   const int row = (warp & 3) * 32 + lane;  // of the tile; TMEM lane
-  const int col0 = (warp >> 2) * S::kCols;
+  const int group = warp >> 2, col0 = group * S::kCols;
+  constexpr int kTileOuts = TOKEN_ROWS ? COLS : kRows;
   if (warp >= S::kEpi) {
     if (S::kSplitRegisters)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegisters));
@@ -192,8 +224,8 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
         tma_prefetch_desc(&xmap);
         int it = 0;
         for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-          const int n0 = static_cast<int>(tile / p.token_tiles) * kRows;
-          const int m0 = static_cast<int>(tile % p.token_tiles) * TOKENS;
+          const int n0 = static_cast<int>(tile / p.token_tiles) * kTileOuts;
+          const int m0 = static_cast<int>(tile % p.token_tiles) * S::kTokens;
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % kStages;
             ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
@@ -201,8 +233,10 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
             if (!ok) break;
             uint8_t* dst = stages + s * S::kStageBytes;
             mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-            tma_load_2d(dst, &wmap, &full[s], kb * kBlock, n0);
-            tma_load_2d(dst + kRows * kBlock, &xmap, &full[s], kb * kBlock, m0);
+            tma_load_2d(dst, TOKEN_ROWS ? &xmap : &wmap, &full[s], kb * kBlock,
+                        TOKEN_ROWS ? m0 : n0);
+            tma_load_2d(dst + kRows * kBlock, TOKEN_ROWS ? &wmap : &xmap, &full[s], kb * kBlock,
+                        TOKEN_ROWS ? n0 : m0);
           }
         }
         drain_stages<kStages>(full, it, p.err);
@@ -210,7 +244,7 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
     } else if (warp == S::kEpi + 1) {
       // ------------------------------ MMA issuer ----------------------------
       if (lane == 0) {
-        const uint32_t idesc = tc::idesc_e4m3(kRows, TOKENS);
+        const uint32_t idesc = tc::idesc_e4m3(kRows, COLS);
         const uint32_t st0 = smem_u32(stages);
         int it = 0;
         for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
@@ -221,12 +255,12 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
                  mbar_wait_bounded(&full[s], (it / kStages) & 1, abort_flag, p.err, kErrWaitFull);
             if (!ok) break;
             tc::fence_after_sync();
-            const uint32_t w = st0 + s * S::kStageBytes;
-            const uint32_t x = w + kRows * kBlock;
+            const uint32_t rows = st0 + s * S::kStageBytes;
+            const uint32_t cols = rows + kRows * kBlock;
 #pragma unroll
             for (int k = 0; k < kBlock / 32; ++k)
-              tc::mma_e4m3(tmem + b * S::kBufferCols, tc::sdesc_sw128(w + k * 32, 16, 1024),
-                           tc::sdesc_sw128(x + k * 32, 16, 1024), idesc, k > 0);
+              tc::mma_e4m3(tmem + b * S::kBufferCols, tc::sdesc_sw128(rows + k * 32, 16, 1024),
+                           tc::sdesc_sw128(cols + k * 32, 16, 1024), idesc, k > 0);
             tc::commit(&empty[s]);
             tc::commit(&acc_full[b]);
           }
@@ -236,44 +270,31 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
         mbar_wait_bounded(mma_idle, 0, abort_flag, p.err, kErrDrain);
       }
     } else if (warp == S::kEpi + 2) {
-      // ---------------------------- scale products --------------------------
-      // kAhead blocks at a time, so that their loads are in flight together.
-      constexpr int kAhead = TOKENS > 128 ? 2 : 4;
-      constexpr int kPer = (TOKENS + 31) / 32;
+      // -------------------------------- scales ------------------------------
       int it = 0;
       for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-        const long long m0 = tile % p.token_tiles * TOKENS;
-        const float* sw = p.w_scales + tile / p.token_tiles * p.ws_row;
-        for (int kb = kb0; kb < kb1 && ok; kb += kAhead) {
-          float v[kAhead][kPer];
+        const long long m0 = tile % p.token_tiles * S::kTokens;
+        const long long n0 = tile / p.token_tiles * kTileOuts;
+        const float* sx = p.x_scales + (m0 + lane) * p.xs_row;
+        const float* sw = p.w_scales + (n0 / 128 + lane) * p.ws_row;
+        const bool has_w = lane < S::kGroups && n0 + lane * 128 < p.n;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int r = it % kScaleRing;
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sc_empty[r], ((it / kScaleRing) & 1) ^ 1,
+                                                         abort_flag, p.err, kErrWaitEmpty));
+          if (!ok) break;
+          float* dst = scales + r * S::kScales;
 #pragma unroll
-          for (int a = 0; a < kAhead; ++a) {
-            if (kb + a >= kb1) break;
-            const float ws = sw[(kb + a) * p.ws_block];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const long long m = m0 + i * 32 + lane;
-              v[a][i] = m < p.m && i * 32 + lane < TOKENS
-                            ? p.x_scales[m * p.xs_row + (kb + a) * p.xs_block] * ws
-                            : 0.f;
-            }
+          for (int i = 0; i < (S::kTokens + 31) / 32; ++i) {
+            const int c = i * 32 + lane;
+            if (c < S::kTokens && m0 + c < p.m)
+              copy_async_4(dst + c, sx + i * 32 * p.xs_row + kb * p.xs_block);
           }
-#pragma unroll
-          for (int a = 0; a < kAhead; ++a) {
-            if (kb + a >= kb1) break;
-            const int r = it % kScaleRing;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sc_empty[r], ((it / kScaleRing) & 1) ^ 1,
-                                                           abort_flag, p.err, kErrWaitEmpty));
-            if (!ok) break;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-              if (i * 32 + lane < TOKENS) scales[r * TOKENS + i * 32 + lane] = v[a][i];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sc_full[r]);
-            ++it;
-          }
+          if (has_w) copy_async_4(dst + S::kTokens + lane, sw + kb * p.ws_block);
+          copy_async_arrive(&sc_full[r]);
         }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else {
     // ------------------------------ epilogue ------------------------------
@@ -295,8 +316,12 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
                                   kErrWaitFull));
         if (!ok) break;
         tc::fence_after_sync();
-        const ulonglong2* sc =
-            reinterpret_cast<const ulonglong2*>(scales + r * TOKENS + col0);
+        const float* sc = scales + r * S::kScales;
+        const float sw = sc[S::kTokens + group];
+        // Tokens as rows: this row's scale.
+        const float s1 = TOKEN_ROWS ? sc[row] * sw : sw;
+        const u64 s2 = pack_f32x2(__float_as_uint(s1), __float_as_uint(s1));
+        const ulonglong2* sx = reinterpret_cast<const ulonglong2*>(sc);
         // The next columns are on their way while these are added.
         constexpr int kStep = S::kStep, kSteps = S::kCols / kStep;
         uint32_t v[2][kStep];
@@ -313,19 +338,65 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
           }
 #pragma unroll
           for (int i = 0; i < kStep / 4; ++i) {
-            const ulonglong2 s2 = sc[c * (kStep / 4) + i];
+            ulonglong2 f = make_ulonglong2(s2, s2);
+            if (!TOKEN_ROWS) {
+              f = sx[c * (kStep / 4) + i];
+              f.x = mul2(f.x, s2);
+              f.y = mul2(f.y, s2);
+            }
             const int a = (c * kStep) / 2 + 2 * i;
-            fma2(acc[a], pack_f32x2(v[c & 1][4 * i], v[c & 1][4 * i + 1]), s2.x);
-            fma2(acc[a + 1], pack_f32x2(v[c & 1][4 * i + 2], v[c & 1][4 * i + 3]), s2.y);
+            fma2(acc[a], pack_f32x2(v[c & 1][4 * i], v[c & 1][4 * i + 1]), f.x);
+            fma2(acc[a + 1], pack_f32x2(v[c & 1][4 * i + 2], v[c & 1][4 * i + 3]), f.y);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_empty[r]);
       }
       if (!ok) break;
-      const long long n = tile / p.token_tiles * kRows + row;
-      const long long m0 = tile % p.token_tiles * TOKENS + col0;
-      if (p.splits == 1) {
+      if (p.splits > 1) {
+        // One tile per CTA: its stages are free, every copy and MMA has finished.
+        float* part = reinterpret_cast<float*>(stages) + col0 * kPartPitch + row;
+#pragma unroll
+        for (int i = 0; i < S::kCols / 2; ++i) {
+          const float2 f = unpack_f32x2(acc[i]);
+          part[2 * i * kPartPitch] = f.x;
+          part[(2 * i + 1) * kPartPitch] = f.y;
+        }
+      } else if (TOKEN_ROWS) {
+        const long long m = tile % p.token_tiles * kRows + row;
+        const long long n0 = tile / p.token_tiles * COLS + col0;
+        if (m < p.m && n0 < p.n) {
+          T* out = reinterpret_cast<T*>(p.out) + m * p.out_stride + n0;
+          const T* bias = reinterpret_cast<const T*>(p.bias);
+#pragma unroll
+          for (int i = 0; i < S::kCols / 16; ++i) {
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float2 pair = unpack_f32x2(acc[8 * i + j]);
+              f[2 * j] = pair.x;
+              f[2 * j + 1] = pair.y;
+            }
+            if (bias) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (n0 + 16 * i + j < p.n) f[j] += to_float<E>(bias[n0 + 16 * i + j]);
+            }
+            if (p.wide_stores && n0 + 16 * i + 16 <= p.n) {
+              uint32_t w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) w[j] = pack2<E>(f[2 * j], f[2 * j + 1]);
+              store_32b(out + 16 * i, w);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (n0 + 16 * i + j < p.n) out[16 * i + j] = from_float<E>(f[j]);
+            }
+          }
+        }
+      } else {
+        const long long n = tile / p.token_tiles * kRows + row;
+        const long long m0 = tile % p.token_tiles * COLS + col0;
         if (n < p.n) {
           const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
           T* out = reinterpret_cast<T*>(p.out) + m0 * p.out_stride + n;
@@ -336,35 +407,28 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
             if (m0 + 2 * i + 1 < p.m) out[(2 * i + 1) * p.out_stride] = from_float<E>(f.y + bias);
           }
         }
-      } else if (TOKENS <= 128) {
-        // One tile per CTA: its stages are free, every copy and MMA has finished.
-        float* part = reinterpret_cast<float*>(stages);
-#pragma unroll
-        for (int i = 0; i < S::kCols / 2; ++i) {
-          const float2 f = unpack_f32x2(acc[i]);
-          part[(col0 + 2 * i) * kRows + row] = f.x;
-          part[(col0 + 2 * i + 1) * kRows + row] = f.y;
-        }
       }
     }
   }
   __syncwarp();  // single-thread roles rejoin their warp
   if (p.splits > 1) {
-    // Join: rank r adds the columns [TOKENS r / splits, ...) of all ranks, in rank order.
+    // Join: rank r adds the tokens [kTokens r / splits, ...) of all ranks, in rank
+    // order; lanes take neighbouring outputs.
     cluster.sync();
     if (warp < S::kEpi && ok) {
-      const long long n = tile0 / p.token_tiles * kRows + row;
-      const long long m0 = tile0 % p.token_tiles * TOKENS;
-      const int c1 = static_cast<int>(min(static_cast<long long>(TOKENS * (rank + 1) / p.splits),
-                                          p.m - m0));
-      float* part = reinterpret_cast<float*>(stages);
-      if (n < p.n) {
-        const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
-        for (int c = TOKENS * rank / p.splits; c < c1; ++c) {
+      const long long n0 = tile0 / p.token_tiles * kTileOuts;
+      const long long m0 = tile0 % p.token_tiles * S::kTokens;
+      const int t1 = static_cast<int>(min(
+          static_cast<long long>(S::kTokens * (rank + 1) / p.splits), p.m - m0));
+      const float* part = reinterpret_cast<const float*>(stages);
+      for (int o = tid; o < kTileOuts && n0 + o < p.n; o += S::kEpi * 32) {
+        const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n0 + o]) : 0.f;
+        for (int t = S::kTokens * rank / p.splits; t < t1; ++t) {
+          const float* at = part + (TOKEN_ROWS ? o * kPartPitch + t : t * kPartPitch + o);
           float sum = 0.f;
-          for (int o = 0; o < p.splits; ++o)
-            sum += *cluster.map_shared_rank(part + c * kRows + row, o);
-          reinterpret_cast<T*>(p.out)[(m0 + c) * p.out_stride + n] = from_float<E>(sum + bias);
+          for (int r = 0; r < p.splits; ++r) sum += *cluster.map_shared_rank(at, r);
+          reinterpret_cast<T*>(p.out)[(m0 + t) * p.out_stride + n0 + o] =
+              from_float<E>(sum + bias);
         }
       }
     }
@@ -379,11 +443,11 @@ __global__ void __launch_bounds__(Shape<TOKENS>::kThreads, Shape<TOKENS>::kCtasP
   }
 }
 
-template <typename E, int TOKENS>
+template <typename E, int COLS, bool TOKEN_ROWS>
 int launch(const CUtensorMap& wmap, const CUtensorMap& xmap, const LinearParams& p, int ctas,
            cudaStream_t stream) {
-  using S = Shape<TOKENS>;
-  auto kern = fp8_linear_kernel<E, TOKENS>;
+  using S = Shape<COLS, TOKEN_ROWS>;
+  auto kern = fp8_linear_kernel<E, COLS, TOKEN_ROWS>;
   const cudaError_t err =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (err != cudaSuccess) return cuda_status(err, "fp8_linear_kernel shared memory");
@@ -412,31 +476,31 @@ int launch(const CUtensorMap& wmap, const CUtensorMap& xmap, const LinearParams&
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, wmap, xmap, p), "fp8_linear_kernel launch");
 }
 
-template <int TOKENS>
+template <int COLS, bool TOKEN_ROWS>
 int launch_any(const b200_fp8_linear_args* a, const void* x, const void* w, LinearParams p,
                int sms, cudaStream_t stream) {
-  const int slots = sms * Shape<TOKENS>::kCtasPerSm;
-  p.token_tiles = static_cast<int>(ceil_div64(a->m, TOKENS));
-  p.tiles = ceil_div64(a->n, kRows) * p.token_tiles;
+  using S = Shape<COLS, TOKEN_ROWS>;
+  const int slots = sms * S::kCtasPerSm;
+  const int tile_outs = TOKEN_ROWS ? COLS : kRows;
+  p.token_tiles = static_cast<int>(ceil_div64(a->m, S::kTokens));
+  p.tiles = ceil_div64(a->n, tile_outs) * p.token_tiles;
   // Splits of K that still fit the CTAs at once, each with two blocks or more.
-  p.splits = 1;
-  if (TOKENS <= 128)
-    p.splits = static_cast<int>(std::max<long long>(
-        1, std::min<long long>({kMaxSplits, slots / p.tiles, p.blocks / 2})));
+  p.splits = static_cast<int>(std::max<long long>(
+      1, std::min<long long>({kMaxSplits, slots / p.tiles, p.blocks / 2})));
   const long long ctas = p.splits > 1 ? p.tiles * p.splits : std::min<long long>(p.tiles, slots);
   const uint64_t wdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->n)};
   const uint64_t xdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->m)};
   const uint64_t wstride[1] = {static_cast<uint64_t>(a->w_stride)};
   const uint64_t xstride[1] = {static_cast<uint64_t>(a->x_stride)};
-  const uint32_t wbox[2] = {kBlock, kRows};
-  const uint32_t xbox[2] = {kBlock, TOKENS};
+  const uint32_t wbox[2] = {kBlock, static_cast<uint32_t>(tile_outs)};
+  const uint32_t xbox[2] = {kBlock, static_cast<uint32_t>(S::kTokens)};
   CUtensorMap wmap, xmap;
   int rc = encode_tensor_map_8b(w, 2, wdims, wstride, wbox, &wmap);
   if (rc == B200_OK) rc = encode_tensor_map_8b(x, 2, xdims, xstride, xbox, &xmap);
   if (rc != B200_OK) return rc;
   return a->dtype == B200_BF16
-             ? launch<BF16, TOKENS>(wmap, xmap, p, static_cast<int>(ctas), stream)
-             : launch<Half, TOKENS>(wmap, xmap, p, static_cast<int>(ctas), stream);
+             ? launch<BF16, COLS, TOKEN_ROWS>(wmap, xmap, p, static_cast<int>(ctas), stream)
+             : launch<Half, COLS, TOKEN_ROWS>(wmap, xmap, p, static_cast<int>(ctas), stream);
 }
 
 }  // namespace
@@ -473,11 +537,16 @@ int launch_fp8_linear(const b200_fp8_linear_args* a, const void* x, const float*
   p.ws_block = a->w_scale_stride_block;
   p.out_stride = a->out_stride;
   p.blocks = static_cast<int>(ceil_div64(a->k, kBlock));
-  if (a->m <= 16) return launch_any<16>(a, x, w, p, info.num_sms, stream);
-  if (a->m <= 32) return launch_any<32>(a, x, w, p, info.num_sms, stream);
-  if (a->m <= 64) return launch_any<64>(a, x, w, p, info.num_sms, stream);
-  if (a->m <= 128) return launch_any<128>(a, x, w, p, info.num_sms, stream);
-  return launch_any<256>(a, x, w, p, info.num_sms, stream);
+  p.wide_stores = a->out_stride % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
+  const int sms = info.num_sms;
+  if (a->m <= 16) return launch_any<16, false>(a, x, w, p, sms, stream);
+  if (a->m <= 32) return launch_any<32, false>(a, x, w, p, sms, stream);
+  if (a->m <= 64) return launch_any<64, false>(a, x, w, p, sms, stream);
+  if (a->m <= 128) return launch_any<128, false>(a, x, w, p, sms, stream);
+  // 256 columns halve what a tile reads of x, if their tiles still fill the SMs.
+  if (ceil_div64(a->m, kRows) * ceil_div64(a->n, 256) >= sms)
+    return launch_any<256, true>(a, x, w, p, sms, stream);
+  return launch_any<128, true>(a, x, w, p, sms, stream);
 }
 
 }  // namespace b200
