@@ -66,8 +66,12 @@ struct Shape {
   static constexpr int kEpi = 4 * kGroups;
   static constexpr int kThreads = (kEpi + 4) * 32;
   static constexpr int kCols = COLS / kGroups;         // columns of an epilogue thread
-  static constexpr int kStep = kCols < 32 ? kCols : 32;  // columns of one TMEM load
-  // 256 columns: 128 sums and 64 loaded values per epilogue thread are more than the
+  // Columns of the TMEM loads, in turn.  128 columns: 32, 16, 32, 16, 32 -- twice 32
+  // do not fit the registers, twice 16 leave more of a load's latency uncovered.
+  static constexpr int kStepA = kCols >= 128 ? 32 : 16, kStepB = 16;
+  static_assert(kCols % (kStepA + kStepB) == 0 || kCols % (kStepA + kStepB) == kStepA,
+                "the loads end with the columns");
+  // 256 columns: 128 sums and 48 loaded values per epilogue thread are more than the
   // 168 registers of 384 threads, so that the other four warps give some of theirs.
   static constexpr bool kSplitRegisters = COLS > 128;
   static constexpr int kEpiRegisters = 224, kOtherRegisters = 56, kLaunchRegisters = 168;
@@ -101,12 +105,11 @@ struct LinearParams {
   const void* bias;
   void* out;
   uint32_t* err;
-  long long m, n;
+  int m, n;
   long long xs_row, xs_block, ws_row, ws_block, out_stride;
   int blocks;  // of K
   int token_tiles;
-  long long tiles;
-  int splits;
+  int tiles, splits;
   int wide_stores;  // 32-byte stores of a token's outputs
 };
 
@@ -152,6 +155,14 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[16]) 
   tc::ld16(taddr, v);
 }
 
+// A bounded wait whose outcome every lane of the warp shares; out of line where it
+// has to wait.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                          uint32_t* err) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, err, kErrWaitFull));
+}
+
 template <typename E, int COLS, bool TOKEN_ROWS>
 __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
                                   Shape<COLS, TOKEN_ROWS>::kCtasPerSm)
@@ -178,8 +189,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
-  const long long tile0 = blockIdx.x / p.splits;
-  const long long tile_step = gridDim.x / p.splits;
+  const int tile0 = blockIdx.x / p.splits, tile_step = gridDim.x / p.splits;
   const int kb0 = static_cast<int>(static_cast<long long>(p.blocks) * rank / p.splits);
   const int kb1 = static_cast<int>(static_cast<long long>(p.blocks) * (rank + 1) / p.splits);
 
@@ -223,9 +233,9 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
         tma_prefetch_desc(&wmap);
         tma_prefetch_desc(&xmap);
         int it = 0;
-        for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-          const int n0 = static_cast<int>(tile / p.token_tiles) * kTileOuts;
-          const int m0 = static_cast<int>(tile % p.token_tiles) * S::kTokens;
+        for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+          const int n0 = tile / p.token_tiles * kTileOuts;
+          const int m0 = tile % p.token_tiles * S::kTokens;
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % kStages;
             ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
@@ -247,7 +257,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
         const uint32_t idesc = tc::idesc_e4m3(kRows, COLS);
         const uint32_t st0 = smem_u32(stages);
         int it = 0;
-        for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+        for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % kStages, b = it % kBuffers;
             ok = mbar_wait_bounded(&acc_empty[b], ((it / kBuffers) & 1) ^ 1, abort_flag, p.err,
@@ -272,9 +282,9 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     } else if (warp == S::kEpi + 2) {
       // -------------------------------- scales ------------------------------
       int it = 0;
-      for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-        const long long m0 = tile % p.token_tiles * S::kTokens;
-        const long long n0 = tile / p.token_tiles * kTileOuts;
+      for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+        const int m0 = tile % p.token_tiles * S::kTokens;
+        const int n0 = tile / p.token_tiles * kTileOuts;
         const float* sx = p.x_scales + (m0 + lane) * p.xs_row;
         const float* sw = p.w_scales + (n0 / 128 + lane) * p.ws_row;
         const bool has_w = lane < S::kGroups && n0 + lane * 128 < p.n;
@@ -301,56 +311,72 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     if (S::kSplitRegisters)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kEpiRegisters));
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + col0;
+    auto release = [&](uint64_t* bar) {  // the accumulator has been read
+      tc::fence_before_sync();
+      if (lane == 0) mbar_arrive(bar);
+    };
     int it = 0;
-    for (long long tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+    for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
       u64 acc[S::kCols / 2];
 #pragma unroll
       for (int i = 0; i < S::kCols / 2; ++i) acc[i] = 0;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int b = it % kBuffers, r = it % kScaleRing;
-        ok = __all_sync(
-            0xffffffffu,
-            mbar_wait_bounded(&sc_full[r], (it / kScaleRing) & 1, abort_flag, p.err,
-                              kErrWaitFull) &&
-                mbar_wait_bounded(&acc_full[b], (it / kBuffers) & 1, abort_flag, p.err,
-                                  kErrWaitFull));
+        ok = warp_wait(&acc_full[b], (it / kBuffers) & 1, abort_flag, p.err);
         if (!ok) break;
         tc::fence_after_sync();
+        const uint32_t base = lane_base + b * S::kBufferCols;
+        uint32_t va[S::kStepA], vb[S::kStepB];
+        load_columns(base, va);
+        // Meanwhile the scales: with tokens as rows, this row's.
+        ok = warp_wait(&sc_full[r], (it / kScaleRing) & 1, abort_flag, p.err);
         const float* sc = scales + r * S::kScales;
         const float sw = sc[S::kTokens + group];
-        // Tokens as rows: this row's scale.
         const float s1 = TOKEN_ROWS ? sc[row] * sw : sw;
         const u64 s2 = pack_f32x2(__float_as_uint(s1), __float_as_uint(s1));
         const ulonglong2* sx = reinterpret_cast<const ulonglong2*>(sc);
-        // The next columns are on their way while these are added.
-        constexpr int kStep = S::kStep, kSteps = S::kCols / kStep;
-        uint32_t v[2][kStep];
-        const uint32_t base = lane_base + b * S::kBufferCols;
-        load_columns(base, v[0]);
+        if (TOKEN_ROWS) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[r]);
+        }
+        auto add = [&](auto& v, int c0) {  // columns c0 .. to the sums
+          constexpr int kN = sizeof(v) / 4;
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          tc::wait_ld(v[c & 1]);
-          if (c + 1 < kSteps) {
-            load_columns(base + (c + 1) * kStep, v[(c + 1) & 1]);
-          } else {  // the buffer has been read
-            tc::fence_before_sync();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
-          }
-#pragma unroll
-          for (int i = 0; i < kStep / 4; ++i) {
+          for (int i = 0; i < kN / 4; ++i) {
             ulonglong2 f = make_ulonglong2(s2, s2);
             if (!TOKEN_ROWS) {
-              f = sx[c * (kStep / 4) + i];
+              f = sx[c0 / 4 + i];
               f.x = mul2(f.x, s2);
               f.y = mul2(f.y, s2);
             }
-            const int a = (c * kStep) / 2 + 2 * i;
-            fma2(acc[a], pack_f32x2(v[c & 1][4 * i], v[c & 1][4 * i + 1]), f.x);
-            fma2(acc[a + 1], pack_f32x2(v[c & 1][4 * i + 2], v[c & 1][4 * i + 3]), f.y);
+            const int a = c0 / 2 + 2 * i;
+            fma2(acc[a], pack_f32x2(v[4 * i], v[4 * i + 1]), f.x);
+            fma2(acc[a + 1], pack_f32x2(v[4 * i + 2], v[4 * i + 3]), f.y);
+          }
+        };
+        // The next columns are on their way while these are added.
+        constexpr int kA = S::kStepA, kB = S::kStepB, kAB = kA + kB;
+#pragma unroll
+        for (int c = 0; c < S::kCols; c += kAB) {
+          tc::wait_ld(va);
+          if (c + kA < S::kCols)
+            load_columns(base + c + kA, vb);
+          else
+            release(acc_empty + b);
+          add(va, c);
+          if (c + kA < S::kCols) {
+            tc::wait_ld(vb);
+            if (c + kAB < S::kCols)
+              load_columns(base + c + kAB, va);
+            else
+              release(acc_empty + b);
+            add(vb, c + kA);
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_empty[r]);
+        if (!TOKEN_ROWS) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[r]);
+        }
       }
       if (!ok) break;
       if (p.splits > 1) {
@@ -363,10 +389,10 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
           part[(2 * i + 1) * kPartPitch] = f.y;
         }
       } else if (TOKEN_ROWS) {
-        const long long m = tile % p.token_tiles * kRows + row;
-        const long long n0 = tile / p.token_tiles * COLS + col0;
+        const int m = tile % p.token_tiles * kRows + row;
+        const int n0 = tile / p.token_tiles * COLS + col0;
         if (m < p.m && n0 < p.n) {
-          T* out = reinterpret_cast<T*>(p.out) + m * p.out_stride + n0;
+          T* out = reinterpret_cast<T*>(p.out) + static_cast<long long>(m) * p.out_stride + n0;
           const T* bias = reinterpret_cast<const T*>(p.bias);
 #pragma unroll
           for (int i = 0; i < S::kCols / 16; ++i) {
@@ -395,8 +421,8 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
           }
         }
       } else {
-        const long long n = tile / p.token_tiles * kRows + row;
-        const long long m0 = tile % p.token_tiles * COLS + col0;
+        const int n = tile / p.token_tiles * kRows + row;
+        const int m0 = tile % p.token_tiles * COLS + col0;
         if (n < p.n) {
           const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
           T* out = reinterpret_cast<T*>(p.out) + m0 * p.out_stride + n;
@@ -416,10 +442,9 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     // order; lanes take neighbouring outputs.
     cluster.sync();
     if (warp < S::kEpi && ok) {
-      const long long n0 = tile0 / p.token_tiles * kTileOuts;
-      const long long m0 = tile0 % p.token_tiles * S::kTokens;
-      const int t1 = static_cast<int>(min(
-          static_cast<long long>(S::kTokens * (rank + 1) / p.splits), p.m - m0));
+      const int n0 = tile0 / p.token_tiles * kTileOuts;
+      const int m0 = tile0 % p.token_tiles * S::kTokens;
+      const int t1 = min(S::kTokens * (rank + 1) / p.splits, p.m - m0);
       const float* part = reinterpret_cast<const float*>(stages);
       for (int o = tid; o < kTileOuts && n0 + o < p.n; o += S::kEpi * 32) {
         const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n0 + o]) : 0.f;
@@ -483,11 +508,14 @@ int launch_any(const b200_fp8_linear_args* a, const void* x, const void* w, Line
   const int slots = sms * S::kCtasPerSm;
   const int tile_outs = TOKEN_ROWS ? COLS : kRows;
   p.token_tiles = static_cast<int>(ceil_div64(a->m, S::kTokens));
-  p.tiles = ceil_div64(a->n, tile_outs) * p.token_tiles;
+  const long long tiles = ceil_div64(a->n, tile_outs) * p.token_tiles;
+  if (tiles > 0x7fffffffLL / kMaxSplits)
+    return set_error(B200_ERR_UNSUPPORTED, "too many output tiles");
+  p.tiles = static_cast<int>(tiles);
   // Splits of K that still fit the CTAs at once, each with two blocks or more.
   p.splits = static_cast<int>(std::max<long long>(
       1, std::min<long long>({kMaxSplits, slots / p.tiles, p.blocks / 2})));
-  const long long ctas = p.splits > 1 ? p.tiles * p.splits : std::min<long long>(p.tiles, slots);
+  const long long ctas = p.splits > 1 ? tiles * p.splits : std::min<long long>(tiles, slots);
   const uint64_t wdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->n)};
   const uint64_t xdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->m)};
   const uint64_t wstride[1] = {static_cast<uint64_t>(a->w_stride)};
@@ -529,8 +557,8 @@ int launch_fp8_linear(const b200_fp8_linear_args* a, const void* x, const float*
   p.bias = bias;
   p.out = out;
   p.err = error_word;
-  p.m = a->m;
-  p.n = a->n;
+  p.m = static_cast<int>(a->m);
+  p.n = static_cast<int>(a->n);
   p.xs_row = a->x_scale_stride_row;
   p.xs_block = a->x_scale_stride_block;
   p.ws_row = a->w_scale_stride_row;
