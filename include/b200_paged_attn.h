@@ -34,7 +34,8 @@
 extern "C" {
 #endif
 
-enum { B200_F16 = 0, B200_BF16 = 1, B200_F32 = 2 }; /* F32: logits of b200_sample_tokens only */
+/* F32: logits of b200_sample_tokens only; E4M3: x of b200_fp8_linear only */
+enum { B200_F16 = 0, B200_BF16 = 1, B200_F32 = 2, B200_E4M3 = 3 };
 enum { B200_I32 = 0, B200_I64 = 1 };
 
 enum {
@@ -439,20 +440,25 @@ B200_API int b200_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_
 
 /* out[m, n] = sum_b x_scales[m, b] w_scales[n / 128, b] sum_{k in block b} x[m, k] w[n, k]
  * (+ bias[n]), blocks of 128 columns, 32-bit sums, rounded once to the output type.
- * x [m, k] and w [n, k] are e4m3 with rows on 16-byte boundaries (x_stride and
- * w_stride multiples of 16); bias (NULL: none) and out have type dtype.
+ * w [n, k] is e4m3 with rows on 16-byte boundaries (w_stride a multiple of 16); bias
+ * (NULL: none) and out have type dtype.  x [m, k] is
+ *   e4m3 (x_dtype B200_E4M3) with x_scales, rows on 16-byte boundaries; or
+ *   16-bit of type dtype (x_dtype = dtype), quantised first as by b200_quantize_fp8
+ *   with block_rows 1, into `workspace`: m * (k rounded up to 16 + 4 * ceil(k / 128))
+ *   bytes on a 16-byte boundary; x_scales and its strides are not used.
  */
 typedef struct {
   int64_t m, n, k;
   int64_t x_stride, w_stride, out_stride; /* elements between rows */
   int64_t x_scale_stride_row, x_scale_stride_block;
   int64_t w_scale_stride_row, w_scale_stride_block;
-  int32_t dtype; /* B200_F16 / B200_BF16 */
+  int32_t dtype;   /* of out: B200_F16 / B200_BF16 */
+  int32_t x_dtype; /* dtype, or B200_E4M3 */
 } b200_fp8_linear_args;
 
 B200_API int b200_fp8_linear(const b200_fp8_linear_args* args, const void* x, const float* x_scales,
                     const void* w, const float* w_scales, const void* bias, void* out,
-                    uint32_t* error_word, void* stream);
+                    void* workspace, size_t workspace_bytes, uint32_t* error_word, void* stream);
 
 /* ------------------------------------------------------------- validation
  * Device-side form of the reference wrappers' validate_inputs checks

@@ -16,7 +16,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libb200_paged_attn.so"
 
-B200_F16, B200_BF16, B200_F32 = 0, 1, 2
+B200_F16, B200_BF16, B200_F32, B200_E4M3 = 0, 1, 2, 3
 B200_I32, B200_I64 = 0, 1
 
 B200_OK = 0
@@ -194,6 +194,7 @@ class Fp8LinearArgs(ctypes.Structure):
         ("w_scale_stride_row", ctypes.c_int64),
         ("w_scale_stride_block", ctypes.c_int64),
         ("dtype", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
     ]
 
 
@@ -243,7 +244,7 @@ _PROTOTYPES = {
     "b200_quantize_fp8": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _i64,
                                          _i64, _vp]),
     "b200_fp8_linear": (ctypes.c_int, [ctypes.POINTER(Fp8LinearArgs), _vp, _vp, _vp, _vp, _vp,
-                                       _vp, _vp, _vp]),
+                                       _vp, _vp, ctypes.c_size_t, _vp, _vp]),
     "b200_read_error_word": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint32), _i32, _vp]),
     "b200_last_error": (ctypes.c_char_p, []),
     "b200_version": (ctypes.c_char_p, []),

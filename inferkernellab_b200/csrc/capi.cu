@@ -239,10 +239,10 @@ int b200_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_t x_strid
 
 int b200_fp8_linear(const b200_fp8_linear_args* args, const void* x, const float* x_scales,
                     const void* w, const float* w_scales, const void* bias, void* out,
-                    uint32_t* error_word, void* stream) {
+                    void* workspace, size_t workspace_bytes, uint32_t* error_word, void* stream) {
   return guarded([&] {
-    return b200::launch_fp8_linear(args, x, x_scales, w, w_scales, bias, out, error_word,
-                                   as_stream(stream));
+    return b200::launch_fp8_linear(args, x, x_scales, w, w_scales, bias, out, workspace,
+                                   workspace_bytes, error_word, as_stream(stream));
   });
 }
 

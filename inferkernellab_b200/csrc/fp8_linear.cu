@@ -42,6 +42,7 @@
 #include "attn_core.cuh"
 #include "common.cuh"
 #include "fp8_linear.h"
+#include "fp8_quant.h"
 #include "host_common.h"
 #include "tcgen05.cuh"
 
@@ -533,24 +534,44 @@ int launch_any(const b200_fp8_linear_args* a, const void* x, const void* w, Line
 
 }  // namespace
 
-int launch_fp8_linear(const b200_fp8_linear_args* a, const void* x, const float* x_scales,
+int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const float* x_scales,
                       const void* w, const float* w_scales, const void* bias, void* out,
-                      uint32_t* error_word, cudaStream_t stream) {
-  if (a == nullptr) return set_error(B200_ERR_INVALID, "null descriptor");
+                      void* workspace, size_t workspace_bytes, uint32_t* error_word,
+                      cudaStream_t stream) {
+  if (args == nullptr) return set_error(B200_ERR_INVALID, "null descriptor");
+  b200_fp8_linear_args quantized = *args;
+  b200_fp8_linear_args* a = &quantized;
   if (a->dtype != B200_F16 && a->dtype != B200_BF16)
     return set_error(B200_ERR_UNSUPPORTED, "the output must be float16 or bfloat16");
+  if (a->x_dtype != B200_E4M3 && a->x_dtype != a->dtype)
+    return set_error(B200_ERR_INVALID, "x must be e4m3 or have the output's type");
   if (a->m < 0 || a->n <= 0 || a->k <= 0)
     return set_error(B200_ERR_INVALID, "rows/outputs/columns out of range");
   if (a->m > 0x7fffff00LL || a->n > 0x7fffff00LL || a->k > 0x7fffff00LL)
     return set_error(B200_ERR_UNSUPPORTED, "sizes are limited to 2^31 - 256");
-  if (a->x_stride % 16 != 0 || a->w_stride % 16 != 0)
+  if (a->w_stride % 16 != 0 || (a->x_dtype == B200_E4M3 && a->x_stride % 16 != 0))
     return set_error(B200_ERR_INVALID, "rows of x and weight must start on 16-byte boundaries");
   if (a->m == 0) return B200_OK;
-  if (!x || !x_scales || !w || !w_scales || !out)
+  if (!x || !w || !w_scales || !out || (a->x_dtype == B200_E4M3 && !x_scales))
     return set_error(B200_ERR_INVALID, "null tensor pointer");
   DeviceInfo info;
-  const int rc = current_device_info(&info);
+  int rc = current_device_info(&info);
   if (rc != B200_OK) return rc;
+  if (a->x_dtype != B200_E4M3) {
+    const int64_t pitch = ceil_div64(a->k, 16) * 16, blocks = ceil_div64(a->k, kBlock);
+    if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+        workspace_bytes < static_cast<size_t>(a->m) * (pitch + 4 * blocks))
+      return set_error(B200_ERR_WORKSPACE, "fp8_linear workspace missing, unaligned or too small");
+    float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + a->m * pitch);
+    rc = launch_quantize_fp8(x, a->m, a->k, a->x_stride, a->x_dtype, 1, workspace, pitch, scales, 1,
+                             a->m, stream);
+    if (rc != B200_OK) return rc;
+    x = workspace;
+    x_scales = scales;
+    a->x_stride = pitch;
+    a->x_scale_stride_row = 1;
+    a->x_scale_stride_block = a->m;
+  }
   LinearParams p;
   p.x_scales = x_scales;
   p.w_scales = w_scales;

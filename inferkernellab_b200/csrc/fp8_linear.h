@@ -10,6 +10,7 @@ namespace b200 {
 
 int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const float* x_scales,
                       const void* w, const float* w_scales, const void* bias, void* out,
-                      uint32_t* error_word, cudaStream_t stream);
+                      void* workspace, size_t workspace_bytes, uint32_t* error_word,
+                      cudaStream_t stream);
 
 }  // namespace b200

@@ -54,8 +54,14 @@ def b200_available() -> bool:
     return True
 
 
+def _raw_stream(index: int) -> int:
+    """Handle of the current stream of CUDA device ``index``, without a Stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _stream_ptr(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return ctypes.c_void_p(_raw_stream(index))
 
 
 def _cache_desc(cache) -> _lib.CacheDesc:
@@ -492,6 +498,15 @@ def rope_append_kv(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     return out
 
 
+def _last_contiguous(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
+    """``t`` with a contiguous last dimension, and its strides."""
+    strides = t.stride()
+    if strides[-1] != 1:
+        t = t.contiguous()
+        strides = t.stride()
+    return t, strides
+
+
 def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                         q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
                         sin: torch.Tensor, cache, slots: torch.Tensor, layer: int = 0, *,
@@ -508,13 +523,15 @@ def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
     """
     if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
         raise ValueError("query must be [T, Hq, D] and key/value [T, Hkv, D]")
-    device = query.device
-    if device.type != "cuda" or any(t.device != device for t in (key, value, q_weight, k_weight,
-                                                                 cos, sin, slots)):
+    index = query.get_device()
+    if (index < 0 or key.get_device() != index or value.get_device() != index
+            or q_weight.get_device() != index or k_weight.get_device() != index
+            or cos.get_device() != index or sin.get_device() != index
+            or slots.get_device() != index):
         raise ValueError("all tensors must be on the same CUDA device")
     layout = cache.layout
     tokens, heads, dim = query.shape
-    if tuple(key.shape) != (tokens, layout.num_kv_heads, layout.head_dim) or dim != layout.head_dim:
+    if key.shape != (tokens, layout.num_kv_heads, layout.head_dim) or dim != layout.head_dim:
         raise ValueError("query/key/value shape does not match cache layout")
     if heads % layout.num_kv_heads != 0:
         raise ValueError("num_heads must be divisible by num_kv_heads")
@@ -532,32 +549,33 @@ def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
     if not eps >= 0.0:
         raise ValueError("eps must be non-negative")
     dtype = cache.k.dtype
-    if any(t.dtype != dtype for t in (query, key, value, q_weight, k_weight, cos, sin)):
+    if (query.dtype != dtype or key.dtype != dtype or value.dtype != dtype
+            or q_weight.dtype != dtype or k_weight.dtype != dtype or cos.dtype != dtype
+            or sin.dtype != dtype):
         raise ValueError("query/key/value/weights/cos/sin must have the cache dtype")
-    if slots.dtype not in _INDEX_CODE:
+    slots_code = _INDEX_CODE.get(slots.dtype)
+    if slots_code is None:
         raise ValueError("slots must use int32 or int64")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
-    elif (out.shape != query.shape or out.dtype != dtype or out.device != device
+        out = torch.empty((tokens, heads, dim), dtype=dtype, device=query.device)
+    elif (out.shape != query.shape or out.dtype != dtype or out.get_device() != index
           or out.stride(-1) != 1):
         raise ValueError("out must match query's shape, dtype and device")
     if tokens == 0:
         return out
-    query, key, value, q_weight, k_weight, cos, sin = (
-        t if t.stride(-1) == 1 else t.contiguous()
-        for t in (query, key, value, q_weight, k_weight, cos, sin))
-    slots = slots.reshape(-1)
-    if not slots.is_contiguous():
-        slots = slots.contiguous()
-    args = _lib.QkNormArgs(tokens, heads, layer, rotary, eps, *query.stride()[:2],
-                           *key.stride()[:2], *value.stride()[:2], *out.stride()[:2],
-                           cos.stride(0), sin.stride(0), _INDEX_CODE[slots.dtype])
+    (query, qs), (key, ks), (value, vs), (cos, cs), (sin, ss), (q_weight, _), (k_weight, _) = map(
+        _last_contiguous, (query, key, value, cos, sin, q_weight, k_weight))
+    if slots.ndim != 1 or slots.stride(0) != 1:
+        slots = slots.reshape(-1).contiguous()
+    os = out.stride()
+    args = _lib.QkNormArgs(tokens, heads, layer, rotary, eps, qs[0], qs[1], ks[0], ks[1], vs[0],
+                           vs[1], os[0], os[1], cs[0], ss[0], slots_code)
     desc = _cache_desc(cache)
     _lib.check(_lib.load().b200_qk_norm_rope_append(
         ctypes.byref(desc), ctypes.byref(args), query.data_ptr(), key.data_ptr(),
         value.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
-        sin.data_ptr(), slots.data_ptr(), out.data_ptr(), _ERROR_WORDS.get(device).data_ptr(),
-        _stream_ptr(device)))
+        sin.data_ptr(), slots.data_ptr(), out.data_ptr(),
+        _ERROR_WORDS.get(query.device).data_ptr(), _raw_stream(index)))
     return out
 
 
@@ -576,38 +594,49 @@ def copy_kv_pages(cache, src, dst, *, tokens=None) -> None:
     device = cache.k.device
     if device.type != "cuda":
         raise ValueError("the cache must live on a CUDA device")
-    layout = cache.layout
-    on_host = [v is None or isinstance(v, (list, tuple)) for v in (src, dst, tokens)]
-    if isinstance(src, (list, tuple)) and isinstance(dst, (list, tuple)):
+    if not (isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor)
+            and (tokens is None or isinstance(tokens, torch.Tensor))):
+        src, dst, tokens = _page_lists(cache.layout, device, src, dst, tokens)
+    code = _INDEX_CODE.get(src.dtype)
+    if code is None or dst.dtype != src.dtype or (tokens is not None and tokens.dtype != src.dtype):
+        raise ValueError("src, dst and tokens must share an int32/int64 dtype")
+    if (src.ndim != 1 or dst.shape != src.shape
+            or (tokens is not None and tokens.shape != src.shape)):
+        raise ValueError("src, dst and tokens must have one entry per page")
+    if src.device != device or dst.device != device or (tokens is not None
+                                                        and tokens.device != device):
+        raise ValueError("src, dst and tokens must be on the cache device")
+    src, dst = src.contiguous(), dst.contiguous()
+    if tokens is not None:
+        tokens = tokens.contiguous()
+    desc = _cache_desc(cache)
+    _lib.check(_lib.load().b200_copy_kv_pages(
+        ctypes.byref(desc), src.data_ptr(), dst.data_ptr(),
+        tokens.data_ptr() if tokens is not None else None, code, src.numel(),
+        _ERROR_WORDS.get(device).data_ptr(), _raw_stream(device.index)))
+
+
+def _page_lists(layout, device, src, dst, tokens):
+    """``copy_kv_pages`` arguments of which some are Python lists, checked, as device tensors."""
+    given = [src, dst] if tokens is None else [src, dst, tokens]
+    listed = [isinstance(v, (list, tuple)) for v in given]
+    if listed[0] and listed[1]:
         if any(not 0 <= b < layout.num_blocks for b in (*src, *dst)):
             raise ValueError("src/dst contain an invalid physical block id")
         if len(set(dst)) != len(dst) or set(dst) & set(src):
             raise ValueError("a page may be the destination of one copy only, and of none that "
                              "reads it")
-    if isinstance(tokens, (list, tuple)) and any(not 0 <= n <= layout.block_size for n in tokens):
+    if tokens is not None and listed[2] and any(not 0 <= n <= layout.block_size for n in tokens):
         raise ValueError("tokens must lie in [0, block_size]")
-    given = [v for v in (src, dst, tokens) if v is not None]
-    if all(on_host):  # one copy to the device
+    if all(listed):  # one copy to the device
         if any(len(v) != len(src) for v in given):
             raise ValueError("src, dst and tokens must have one entry per page")
         given = list(torch.tensor([list(v) for v in given], dtype=torch.int32).to(device))
     else:
-        dtypes = {v.dtype for v in given if isinstance(v, torch.Tensor)}
-        if len(dtypes) != 1 or not dtypes <= set(_INDEX_CODE):
-            raise ValueError("src, dst and tokens must share an int32/int64 dtype")
-        index = dtypes.pop()
+        index = next(v.dtype for v in given if isinstance(v, torch.Tensor))
         given = [torch.tensor(v, dtype=index).to(device) if isinstance(v, (list, tuple)) else v
                  for v in given]
-    if any(v.ndim != 1 or v.shape != given[0].shape for v in given):
-        raise ValueError("src, dst and tokens must have one entry per page")
-    if any(v.device != device for v in given):
-        raise ValueError("src, dst and tokens must be on the cache device")
-    given = [v if v.is_contiguous() else v.contiguous() for v in given]
-    desc = _cache_desc(cache)
-    _lib.check(_lib.load().b200_copy_kv_pages(
-        ctypes.byref(desc), given[0].data_ptr(), given[1].data_ptr(),
-        given[2].data_ptr() if tokens is not None else None, _INDEX_CODE[given[0].dtype],
-        given[0].numel(), _ERROR_WORDS.get(device).data_ptr(), _stream_ptr(device)))
+    return given[0], given[1], given[2] if tokens is not None else None
 
 
 def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor, *,
@@ -618,26 +647,29 @@ def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor, *,
     stays maps to itself).  Negative entries (unused columns) stay as they are; an entry past
     ``page_map`` stays and sets the device error word.  ``out`` may be ``block_tables`` itself.
     """
-    if block_tables.ndim != 2 or block_tables.device.type != "cuda":
+    index = block_tables.get_device()
+    if block_tables.ndim != 2 or index < 0:
         raise ValueError("block_tables must be a 2-D CUDA tensor")
-    if block_tables.dtype not in _INDEX_CODE:
+    code = _INDEX_CODE.get(block_tables.dtype)
+    if code is None:
         raise ValueError("block_tables must use int32 or int64")
-    if (page_map.ndim != 1 or page_map.dtype != torch.int32 or page_map.numel() == 0
-            or page_map.device != block_tables.device):
+    pages = page_map.numel()
+    if (page_map.ndim != 1 or page_map.dtype != torch.int32 or pages == 0
+            or page_map.get_device() != index):
         raise ValueError("page_map must be a 1-D int32 tensor on the tables' device")
+    rows, width = block_tables.shape
     if out is None:
-        out = torch.empty(block_tables.shape, dtype=block_tables.dtype, device=block_tables.device)
+        out = torch.empty((rows, width), dtype=block_tables.dtype, device=block_tables.device)
     elif (out.shape != block_tables.shape or out.dtype != block_tables.dtype
-          or out.device != block_tables.device or (out.shape[1] > 1 and out.stride(1) != 1)):
+          or out.get_device() != index or (width > 1 and out.stride(1) != 1)):
         raise ValueError("out must match block_tables, with contiguous rows")
     if block_tables.stride(1) != 1:
         block_tables = block_tables.contiguous()
     page_map = page_map.contiguous()
     _lib.check(_lib.load().b200_remap_block_tables(
-        block_tables.data_ptr(), _INDEX_CODE[block_tables.dtype], block_tables.stride(0),
-        block_tables.shape[0], block_tables.shape[1], page_map.data_ptr(), page_map.numel(),
-        out.data_ptr(), out.stride(0), _ERROR_WORDS.get(block_tables.device).data_ptr(),
-        _stream_ptr(block_tables.device)))
+        block_tables.data_ptr(), code, block_tables.stride(0), rows, width, page_map.data_ptr(),
+        pages, out.data_ptr(), out.stride(0), _ERROR_WORDS.get(block_tables.device).data_ptr(),
+        _raw_stream(index)))
     return out
 
 

@@ -14,27 +14,28 @@ import math
 import torch
 
 from . import _lib
-from .ops import _stream_ptr
+from .ops import _raw_stream
 
 _LOGITS_CODE = {torch.float16: _lib.B200_F16, torch.bfloat16: _lib.B200_BF16,
                 torch.float32: _lib.B200_F32}
 
 
-def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dtype, default,
-             check):
-    """(device pointer or None, scalar) of a setting given as a number or one entry per row."""
+def _number(value, name: str, off, check):
+    """A setting given as a number (``None``: off), checked."""
     if value is None:
-        return None, None, default
-    if isinstance(value, torch.Tensor) and value.ndim > 0:
-        if value.shape != (rows,) or value.dtype != dtype or value.device != device:
-            raise ValueError(f"{name} must hold one {str(dtype)[6:]} entry per row on the logits "
-                             "device")
-        value = value if value.is_contiguous() else value.contiguous()
-        return value, value.data_ptr(), default
-    value = type(default)(value)
+        return off
+    value = type(off)(value)
     if not check(value):
         raise ValueError(f"{name} is out of range: {value}")
-    return None, None, value
+    return value
+
+
+def _per_row(value: torch.Tensor, name: str, uniforms: torch.Tensor, dtype) -> torch.Tensor:
+    """A setting given as one entry per row, contiguous."""
+    if (value.dtype != dtype or value.shape != uniforms.shape
+            or value.get_device() != uniforms.get_device()):
+        raise ValueError(f"{name} must hold one {str(dtype)[6:]} entry per row on the logits device")
+    return value if value.is_contiguous() else value.contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=None,
@@ -57,7 +58,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1
     probabilities of the token under the temperature alone and among the kept tokens (those of
     temperature 1 where it is 0).  Nothing is read back to the host.
     """
-    if logits.ndim != 2 or logits.device.type != "cuda":
+    index = logits.get_device()
+    if logits.ndim != 2 or index < 0:
         raise ValueError("logits must be a CUDA tensor with shape [B, V]")
     code = _LOGITS_CODE.get(logits.dtype)
     if code is None:
@@ -65,26 +67,41 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1
     rows, vocab = logits.shape
     if vocab <= 0:
         raise ValueError("logits must have at least one column")
-    device = logits.device
-    if uniforms.shape != (rows,) or uniforms.dtype != torch.float32 or uniforms.device != device:
+    f32 = torch.float32
+    if uniforms.dtype != f32 or uniforms.shape != (rows,) or uniforms.get_device() != index:
         raise ValueError("uniforms must hold one float32 entry per row on the logits device")
-    if logits.stride(1) != 1:
+    row_stride, column_stride = logits.stride()
+    if column_stride != 1:
         logits = logits.contiguous()
+        row_stride = vocab
     if not uniforms.is_contiguous():
         uniforms = uniforms.contiguous()
-    f32 = torch.float32
-    # The first of each triple keeps a contiguous copy alive until the launch.
-    t_keep, t_ptr, t = _setting(temperature, "temperature", rows, device, f32, 1.0,
-                                lambda v: 0.0 <= v < math.inf)
-    k_keep, k_ptr, k = _setting(top_k, "top_k", rows, device, torch.int32, 0,
-                                lambda v: 0 <= v < 2 ** 31)
-    p_keep, p_ptr, p = _setting(top_p, "top_p", rows, device, f32, 1.0, lambda v: 0.0 < v <= 1.0)
-    m_keep, m_ptr, m = _setting(min_p, "min_p", rows, device, f32, 0.0, lambda v: 0.0 <= v <= 1.0)
-    tokens = torch.empty(rows, dtype=torch.int64, device=device)
-    logprobs = torch.empty((2, rows), dtype=f32, device=device)
-    args = _lib.SampleArgs(rows, logits.stride(0), vocab, code, t, k, p, m)
-    out = logprobs.data_ptr()
+    t, k, p, m = 1.0, 0, 1.0, 0.0
+    t_ptr = k_ptr = p_ptr = m_ptr = None
+    if isinstance(temperature, torch.Tensor):
+        temperature = _per_row(temperature, "temperature", uniforms, f32)
+        t_ptr = temperature.data_ptr()
+    else:
+        t = _number(temperature, "temperature", 1.0, lambda v: 0.0 <= v < math.inf)
+    if isinstance(top_k, torch.Tensor):
+        top_k = _per_row(top_k, "top_k", uniforms, torch.int32)
+        k_ptr = top_k.data_ptr()
+    else:
+        k = _number(top_k, "top_k", 0, lambda v: 0 <= v < 2 ** 31)
+    if isinstance(top_p, torch.Tensor):
+        top_p = _per_row(top_p, "top_p", uniforms, f32)
+        p_ptr = top_p.data_ptr()
+    else:
+        p = _number(top_p, "top_p", 1.0, lambda v: 0.0 < v <= 1.0)
+    if isinstance(min_p, torch.Tensor):
+        min_p = _per_row(min_p, "min_p", uniforms, f32)
+        m_ptr = min_p.data_ptr()
+    else:
+        m = _number(min_p, "min_p", 0.0, lambda v: 0.0 <= v <= 1.0)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs, sampling = torch.empty_like(uniforms), torch.empty_like(uniforms)
+    args = _lib.SampleArgs(rows, row_stride, vocab, code, t, k, p, m)
     _lib.check(_lib.load().b200_sample_tokens(
         ctypes.byref(args), logits.data_ptr(), uniforms.data_ptr(), t_ptr, k_ptr, p_ptr, m_ptr,
-        tokens.data_ptr(), out, out + 4 * rows, _stream_ptr(device)))
-    return tokens, logprobs[0], logprobs[1]
+        tokens.data_ptr(), logprobs.data_ptr(), sampling.data_ptr(), _raw_stream(index)))
+    return tokens, logprobs, sampling
