@@ -144,8 +144,9 @@ struct Vec<float> {
     v.y = fmaxf(v.y, -INFINITY);
     v.z = fmaxf(v.z, -INFINITY);
     v.w = fmaxf(v.w, -INFINITY);
-    return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+    return largest();
   }
+  __device__ float largest() const { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
 };
 
 template <typename L, typename L2>
@@ -160,6 +161,9 @@ struct Vec16 {
     low.x = low.y = L(-INFINITY);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = __hmax2(v[i], low);
+    return largest();
+  }
+  __device__ float largest() const {
     const L2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
     return fmaxf(static_cast<float>(m.x), static_cast<float>(m.y));
   }
@@ -451,18 +455,22 @@ class Row {
     const int places = kList / ranks;
     if (thread_max >= limit) {
       Shared* home = at(0);
-      each([&](int token, float l) {
-        if (l >= limit) {
+      for (int v = run0 + lane; v < run1; v += 32) {
+        const V x = raw[v];
+        if (x.largest() < limit) continue;
+#pragma unroll 1
+        for (int i = 0; i < kN; ++i) {
+          const float l = reinterpret_cast<const L*>(raw + v)[i];
+          if (l < limit) continue;
           const float w = weight(l);
-          if (w >= min_p && w > 0.f) {
-            const int to = atomicAdd(&s.local_listed, 1);
-            if (to < places) {
-              home->list[rank * places + to] = entry(w, token);
-              home->list_logit[rank * places + to] = l;
-            }
+          if (w < min_p || w == 0.f) continue;
+          const int to = atomicAdd(&s.local_listed, 1);
+          if (to < places) {
+            home->list[rank * places + to] = entry(w, origin + v * kN + i);
+            home->list_logit[rank * places + to] = l;
           }
         }
-      });
+      }
     }
     __syncthreads();
     if (tid < ranks) at(tid)->listed_of[rank] = s.local_listed;
@@ -481,10 +489,13 @@ class Row {
       const int from = tid + i * kThreads;
       n = 0;
       to[i] = -1;
-      for (int r = 0; r < ranks; ++r) {
-        if (from / places == r && from % places < s.listed_of[r]) to[i] = n + from % places;
-        n += s.listed_of[r];
-      }
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < ranks) {
+          const int at = from - r * places, of = s.listed_of[r];
+          if (at >= 0 && at < of) to[i] = n + at;  // of <= places
+          n += of;
+        }
       if (to[i] >= 0) {
         e[i] = s.list[from];
         l[i] = s.list_logit[from];
@@ -580,58 +591,65 @@ class Row {
     return q;
   }
 
-  template <bool kWarp, typename T>
-  __device__ T sum_over(T v, T* red) {  // of the warp, or of the block
+  // Barrier of the first `warps` warps, and a sum over their threads.
+  __device__ void sync_warps(int warps) {
+    if (warps == 1)
+      __syncwarp();
+    else
+      named_bar_sync(1, warps * 32);
+  }
+  template <typename T>
+  __device__ T sum_over(int warps, T v, T* red) {
     v = warp_sum(v);
-    if (kWarp) return v;
-    __syncthreads();
+    if (warps == 1) return v;
     if (lane == 0) red[warp] = v;
-    __syncthreads();
-    v = 0;
-    for (int i = 0; i < kWarps; ++i) v += red[i];
+    sync_warps(warps);
+    v = warp_sum(lane < warps ? red[lane] : T(0));
+    sync_warps(warps);
     return v;
   }
 
   // The cut and the draw among the first n list entries (rank 0), by counting for
-  // each entry what precedes it: of one warp if n <= 32, else of the block.
-  template <bool kWarp, typename F>
+  // each entry what precedes it; only the warps that hold entries take part.
+  template <typename F>
   __device__ void finish(int n, int top_k, bool cut_p, bool of_list, F&& top_p_target, u64 mass,
                          bool greedy, float u, long long b, double sum) {
+    const int warps = (n + 31) / 32;
+    if (warp >= warps) return;
     const u64 mine = tid < n ? s.list[tid] : 0;
     const uint32_t key = static_cast<uint32_t>(mine >> 32);
     const uint32_t q = mass_of_key(key);
     int rank_of = 0;
     u64 before = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) {
       const u64 o = s.list[j];
-      if (o > mine) {
-        ++rank_of;
-        before += mass_of_key(static_cast<uint32_t>(o >> 32));
-      }
+      const uint32_t oq = mass_of_key(static_cast<uint32_t>(o >> 32));
+      rank_of += o > mine;
+      before += o > mine ? oq : 0;
     }
     bool kept = tid < n && rank_of < top_k;
     if (cut_p) {
-      if (of_list) mass = sum_over<kWarp>(static_cast<u64>(kept ? q : 0), s.scan_mass);
+      if (of_list) mass = sum_over(warps, static_cast<u64>(kept ? q : 0), s.scan_mass);
       kept = kept && before < top_p_target(mass);
     }
     const double kept_sum =
-        sum_over<kWarp>(static_cast<double>(kept ? __uint_as_float(key) : 0.f), s.red_d);
+        sum_over(warps, static_cast<double>(kept ? __uint_as_float(key) : 0.f), s.red_d);
     if (greedy) {  // the first largest logit, which is always kept
       if (tid == 0) write(b, first_largest(), m, sum, kept_sum);
       return;
     }
-    const u64 t = draw_target(u, sum_over<kWarp>(static_cast<u64>(kept ? q : 0), s.scan_mass));
+    const u64 t = draw_target(u, sum_over(warps, static_cast<u64>(kept ? q : 0), s.scan_mass));
     // Kept entries alone, then what precedes mine in order of index (~index falls).
+    sync_warps(warps);
     if (tid < n && !kept) s.list[tid] = 0;
-    if (kWarp)
-      __syncwarp();
-    else
-      __syncthreads();
+    sync_warps(warps);
     before = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) {
       const u64 o = s.list[j];
-      if (static_cast<uint32_t>(o) > static_cast<uint32_t>(mine))
-        before += mass_of_key(static_cast<uint32_t>(o >> 32));
+      const uint32_t oq = mass_of_key(static_cast<uint32_t>(o >> 32));
+      before += static_cast<uint32_t>(o) > static_cast<uint32_t>(mine) ? oq : 0;
     }
     if (kept && before <= t && t < before + q)
       write(b, static_cast<int>(~static_cast<uint32_t>(mine)), s.list_logit[tid], sum, kept_sum);
@@ -657,7 +675,7 @@ class Row {
       e[i] = at < kept ? s.list[at] : 0;
       kept_sum += __uint_as_float(static_cast<uint32_t>(e[i] >> 32));
     }
-    kept_sum = sum_over<false>(kept_sum, s.red_d);
+    kept_sum = sum_over(kWarps, kept_sum, s.red_d);
     if (greedy) {
       if (tid == 0) write(b, first_largest(), m, sum, kept_sum);
       return;
@@ -692,7 +710,7 @@ class Row {
   __device__ void add_to_bin(int bin, uint32_t q) {
     atomicAdd(&s.count[bin], 1u);
     atomicAdd(&s.low[bin], q & 0xffffu);
-    atomicAdd(&s.high[bin], q >> 16);
+    if (q >> 16) atomicAdd(&s.high[bin], q >> 16);
   }
 
   // The bin of the row's histogram in which `target` is reached, counted from the
@@ -806,10 +824,21 @@ class Row {
     return true;
   }
 
+  // A logit that is surely below (side -1) or above (1) those of weight `key`: past
+  // it by more than the rounding of exp and of its argument.
+  __device__ float logit_near(uint32_t key, float side) const {
+    const float w = __uint_as_float(key);
+    if (m == INFINITY || w < 1e-37f) return side < 0.f ? -INFINITY : INFINITY;
+    const float x = logf(w) / inv;
+    return m + x + side * (1e-4f * fabsf(x) + 1e-4f / inv + 1e-6f * fabsf(m));
+  }
+
   // f(token, key) for the tokens that pass min_p with keys in [lo, lo + size).
   template <typename F>
   __device__ void each_in(uint32_t lo, uint32_t size, F&& f) {
+    const float low = logit_near(lo, -1.f), high = logit_near(lo + size, 1.f);
     each([&](int token, float l) {
+      if (l < low || l > high) return;
       const float w = weight(l);
       const uint32_t key = __float_as_uint(w);
       if (key - lo < size && w >= min_p && in_slice(token)) f(token, key);
@@ -1017,13 +1046,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (rank != 0) return;
       const int n = row.close_list();
       const u64 mass = few || !cut_p ? 0 : row.row_mass();
-      if (n <= 32) {
-        if (warp == 0)
-          row.template finish<true>(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy,
-                                    u, b, sum);
-      } else if (n <= kCounted) {
-        row.template finish<false>(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy, u,
-                                   b, sum);
+      if (n <= kCounted) {
+        row.finish(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy, u, b, sum);
       } else {
         row.finish_sorted(n, cut_k ? top_k : n, cut_p, few, top_p_target, mass, greedy, u, b,
                           logits, sum);
@@ -1049,7 +1073,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     __syncthreads();  // s.cut has been read
     if (row.cut_at(kMass, top_p_target(cut.mass), pass, mass)) cut = s.cut;
   }
+  const float low = row.logit_near(cut.key, -1.f);
   auto kept_weight = [&](int token, float l) {
+    if (l < low) return 0.f;
     const float w = row.weight(l);
     const uint32_t key = __float_as_uint(w);
     return key > cut.key || (key == cut.key && token <= cut.index) ? w : 0.f;
