@@ -517,29 +517,61 @@ class Row {
   }
 
   // ------------------------------------------------------------- the list
-  // Sorts the first n list entries, largest first (rank 0; the rest is cleared).
+  // One bitonic step of a lane's entry `x` of index `e` with the one j lanes away.
+  __device__ static u64 exchanged(u64 x, int e, int k, int j) {
+    const u64 y = __shfl_xor_sync(0xffffffffu, x, j);
+    const bool take_larger = ((e & k) == 0) == ((e & j) == 0);
+    return (y > x) == take_larger ? y : x;
+  }
+
+  // Sorts the first n list entries, largest first (rank 0; the rest up to the next
+  // power of two is cleared).  Bitonic: a warp holds 64 neighbouring entries in
+  // registers, so that only the steps over 64 and more go through shared memory.
   __device__ void sort_list(int n) {
-    int size = 2;
+    int size = 64;
     while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
-    __syncthreads();
-    const bool small = size <= 64;  // one warp, two entries a lane
-    if (!small || warp == 0) {
-      for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
+    const bool mine = warp * 64 < size;
+    const int ea = warp * 64 + lane, eb = ea + 32;
+    u64 a = mine && ea < n ? s.list[ea] : 0, b = mine && eb < n ? s.list[eb] : 0;
+    for (int k = 2; k <= size; k *= 2) {
+      if (k > 64) {
+        __syncthreads();
+        if (mine) {
+          s.list[ea] = a;
+          s.list[eb] = b;
+        }
+        for (int j = k / 2; j >= 64; j /= 2) {
+          __syncthreads();
           if (tid < size / 2) {
-            const int a = 2 * tid - (tid & (j - 1)), b = a + j;
-            const u64 x = s.list[a], y = s.list[b];
-            if ((x < y) == ((a & k) == 0)) {
-              s.list[a] = y;
-              s.list[b] = x;
+            const int p0 = 2 * tid - (tid & (j - 1)), p1 = p0 + j;
+            const u64 x = s.list[p0], y = s.list[p1];
+            if ((x < y) == ((p0 & k) == 0)) {
+              s.list[p0] = y;
+              s.list[p1] = x;
             }
           }
-          if (small)
-            __syncwarp();
-          else
-            __syncthreads();
         }
+        __syncthreads();
+        if (mine) {
+          a = s.list[ea];
+          b = s.list[eb];
+        }
+      }
+      if (!mine) continue;
+      if (k >= 64 && (a < b) == ((ea & k) == 0)) {  // 32 apart: both in this lane
+        const u64 x = a;
+        a = b;
+        b = x;
+      }
+      for (int j = min(k, 32) / 2; j > 0; j /= 2) {
+        a = exchanged(a, ea, k, j);
+        b = exchanged(b, eb, k, j);
+      }
+    }
+    __syncthreads();
+    if (mine) {
+      s.list[ea] = a;
+      s.list[eb] = b;
     }
     __syncthreads();
   }
