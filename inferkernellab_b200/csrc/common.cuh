@@ -161,6 +161,30 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+// The same into this CTA's shared memory, completing on a barrier of either CTA of
+// the pair (`bar`: its shared::cluster address).  No multicast.
+__device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map,
+                                                 uint32_t bar, int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+// shared::cluster address of `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+// Arrive on a barrier of another CTA of the cluster.  Release at CTA scope: it orders
+// this thread's TMEM reads (completed by tcgen05.wait::ld), not memory that the other
+// CTA would read; at cluster scope the arrival waits for all outstanding stores.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // Tiled bulk-tensor stores shared -> global (bulk async-group completion):
 // issue, then bulk_commit_group(), then bulk_wait_group_read0() before the
 // shared memory is reused or the CTA exits.  Generic-proxy writes of the

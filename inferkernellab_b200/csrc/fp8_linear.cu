@@ -12,9 +12,9 @@
 // add to sums in registers while the tensor core fills the next buffer.
 //
 // Orientation.  An epilogue thread owns one row of the accumulator (a TMEM lane).
-//   Many tokens: tokens are the rows (MMA M = 128) and 128 or 256 outputs the
-//   columns, so that a thread has one scale product per block and 128 outputs, and
-//   writes neighbouring outputs of its token.  (With the outputs as rows the scales
+//   Many tokens: tokens are the rows and 128 or 256 outputs the columns, so that a
+//   thread has one scale product per block and 128 outputs, and writes neighbouring
+//   outputs of its token.  (With the outputs as rows the scales
 //   differ per column; reading 256 of them from shared memory took twice the MMAs'
 //   time, since a load returns 128 bytes a clock even where all lanes read the same.)
 //   Few tokens (up to 128): outputs are the rows and the tokens the columns, 16 to
@@ -25,6 +25,11 @@
 //   warp kEpi          TMA producer: both tiles of a block per stage
 //   warp kEpi + 1      MMA issuer (one thread)
 //   warp kEpi + 2      scales of the blocks ahead, by asynchronous copies
+//
+// Pairs.  With 256 columns, two CTAs share a tile of 256 x 256 (cta_group::2): each
+// loads its 128 rows and half of the columns, 32 KB a block instead of 48.  Alone, a
+// CTA's tile of 128 x 256 asks 96 KB a block of shared memory (48 written, 48 read by
+// the MMAs), which at 128 bytes a clock is 1.5 times the MMAs' 512 clocks.
 //
 // Work: tiles of 128 rows x COLS columns, tokens innermost so that neighbouring
 // CTAs share weight rows in L2.  CTAs are persistent.  Where tiles are fewer than
@@ -79,12 +84,14 @@ struct Shape {
   static_assert(kEpi * kEpiRegisters + 4 * kOtherRegisters <= (kEpi + 4) * kLaunchRegisters ||
                     !kSplitRegisters,
                 "what the epilogue takes is what the other warps give");
-  static constexpr int kStageBytes = (kRows + COLS) * kBlock;
+  static constexpr bool kPair = COLS > 128;
+  static constexpr int kLoadCols = kPair ? COLS / 2 : COLS;  // columns that a CTA loads
+  static constexpr int kStageBytes = (kRows + kLoadCols) * kBlock;
   // Up to 64 columns a CTA takes under half an SM, so that two share it: the
   // product is then bound by the weight's bytes, and 296 CTAs spread them
   // better than 148.
   static constexpr int kCtasPerSm = COLS <= 64 ? 2 : 1;
-  static constexpr int kStages = COLS <= 32 ? 5 : COLS <= 64 ? 4 : COLS <= 128 ? 6 : 4;
+  static constexpr int kStages = COLS <= 32 ? 5 : COLS <= 64 ? 4 : 6;
   static constexpr int kBuffers = COLS > 128 ? 2 : 4;  // accumulators
   static constexpr int kBufferCols = COLS < 32 ? 32 : COLS;
   static constexpr int kTmemCols = kBuffers * kBufferCols;
@@ -95,7 +102,7 @@ struct Shape {
   static constexpr int kBars = 2 * kStages + 2 * kBuffers + 2 * kScaleRing + 1;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleBytes + kBars * 8 + 16;
   static_assert(kTmemCols <= 512 / kCtasPerSm, "TMEM columns");
-  static_assert(kPartPitch * COLS * 4 <= kStages * kStageBytes,
+  static_assert(kPartPitch * COLS * 4 <= kStages * kStageBytes || kPair,
                 "the split sums reuse the stages");
   static_assert(kSmem <= 227 * 1024 / kCtasPerSm - 1024, "shared memory");
 };
@@ -190,9 +197,12 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
-  const int tile0 = blockIdx.x / p.splits, tile_step = gridDim.x / p.splits;
-  const int kb0 = static_cast<int>(static_cast<long long>(p.blocks) * rank / p.splits);
-  const int kb1 = static_cast<int>(static_cast<long long>(p.blocks) * (rank + 1) / p.splits);
+  constexpr bool kPair = S::kPair;
+  const int per_tile = kPair ? 2 : p.splits;  // CTAs of a tile
+  const int tile0 = blockIdx.x / per_tile, tile_step = gridDim.x / per_tile;
+  const int part = kPair ? 0 : rank;  // of K
+  const int kb0 = static_cast<int>(static_cast<long long>(p.blocks) * part / p.splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.blocks) * (part + 1) / p.splits);
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -201,7 +211,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     }
     for (int i = 0; i < kBuffers; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], S::kEpi);
+      mbar_init(&acc_empty[i], kPair ? 2 * S::kEpi : S::kEpi);  // of a pair: rank 0's is used
     }
     for (int i = 0; i < kScaleRing; ++i) {
       mbar_init(&sc_full[i], 32);  // every lane's copies
@@ -212,11 +222,17 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     fence_mbar_init();
   }
   if (warp == S::kEpi + 1) {
-    tc::tmem_alloc(tmem_slot, S::kTmemCols);
-    tc::tmem_relinquish();
+    if (kPair) {
+      tc::tmem_alloc_pair(tmem_slot, S::kTmemCols);
+      tc::tmem_relinquish_pair();
+    } else {
+      tc::tmem_alloc(tmem_slot, S::kTmemCols);
+      tc::tmem_relinquish();
+    }
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (kPair) cluster.sync();  // the other CTA's barriers are in place, too
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -225,6 +241,8 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
   const int row = (warp & 3) * 32 + lane;  // of the tile; TMEM lane
   const int group = warp >> 2, col0 = group * S::kCols;
   constexpr int kTileOuts = TOKEN_ROWS ? COLS : kRows;
+  constexpr int per_pair = kPair ? 2 : 1;  // token tiles of a CTA pair
+  const int pair_rank = kPair ? rank : 0;
   if (warp >= S::kEpi) {
     if (S::kSplitRegisters)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegisters));
@@ -235,27 +253,40 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
         tma_prefetch_desc(&xmap);
         int it = 0;
         for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-          const int n0 = tile / p.token_tiles * kTileOuts;
-          const int m0 = tile % p.token_tiles * S::kTokens;
+          const int n0 = tile / p.token_tiles * kTileOuts + (kPair ? rank * S::kLoadCols : 0);
+          const int m0 = (tile % p.token_tiles * per_pair + pair_rank) * S::kTokens;
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % kStages;
             ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
                                    kErrWaitEmpty);
             if (!ok) break;
             uint8_t* dst = stages + s * S::kStageBytes;
-            mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-            tma_load_2d(dst, TOKEN_ROWS ? &xmap : &wmap, &full[s], kb * kBlock,
-                        TOKEN_ROWS ? m0 : n0);
-            tma_load_2d(dst + kRows * kBlock, TOKEN_ROWS ? &wmap : &xmap, &full[s], kb * kBlock,
-                        TOKEN_ROWS ? n0 : m0);
+            if (kPair) {  // both CTAs' bytes arrive on rank 0's barrier
+              const uint32_t bar = cluster_address(&full[s], 0);
+              if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);
+              tma_load_2d_pair(dst, &xmap, bar, kb * kBlock, m0);
+              tma_load_2d_pair(dst + kRows * kBlock, &wmap, bar, kb * kBlock, n0);
+            } else {
+              mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+              tma_load_2d(dst, TOKEN_ROWS ? &xmap : &wmap, &full[s], kb * kBlock,
+                          TOKEN_ROWS ? m0 : n0);
+              tma_load_2d(dst + kRows * kBlock, TOKEN_ROWS ? &wmap : &xmap, &full[s], kb * kBlock,
+                          TOKEN_ROWS ? n0 : m0);
+            }
           }
         }
-        drain_stages<kStages>(full, it, p.err);
+        if (!kPair || rank == 0) drain_stages<kStages>(full, it, p.err);
+        // After an abort, rank 1's copies have no barrier of its own to wait for: far
+        // longer than any copy takes.
+        if (kPair && !ok)
+          for (const unsigned long long t0 = global_timer_ns();
+               global_timer_ns() - t0 < 2000000ull;) {
+          }
       }
     } else if (warp == S::kEpi + 1) {
       // ------------------------------ MMA issuer ----------------------------
-      if (lane == 0) {
-        const uint32_t idesc = tc::idesc_e4m3(kRows, COLS);
+      if (lane == 0 && (!kPair || rank == 0)) {
+        const uint32_t idesc = tc::idesc_e4m3(kPair ? 2 * kRows : kRows, COLS);
         const uint32_t st0 = smem_u32(stages);
         int it = 0;
         for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
@@ -268,23 +299,37 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
             tc::fence_after_sync();
             const uint32_t rows = st0 + s * S::kStageBytes;
             const uint32_t cols = rows + kRows * kBlock;
+            const uint32_t d = tmem + b * S::kBufferCols;
 #pragma unroll
-            for (int k = 0; k < kBlock / 32; ++k)
-              tc::mma_e4m3(tmem + b * S::kBufferCols, tc::sdesc_sw128(rows + k * 32, 16, 1024),
-                           tc::sdesc_sw128(cols + k * 32, 16, 1024), idesc, k > 0);
-            tc::commit(&empty[s]);
-            tc::commit(&acc_full[b]);
+            for (int k = 0; k < kBlock / 32; ++k) {
+              const uint64_t da = tc::sdesc_sw128(rows + k * 32, 16, 1024);
+              const uint64_t db = tc::sdesc_sw128(cols + k * 32, 16, 1024);
+              if (kPair)
+                tc::mma_e4m3_pair(d, da, db, idesc, k > 0);
+              else
+                tc::mma_e4m3(d, da, db, idesc, k > 0);
+            }
+            if (kPair) {
+              tc::commit_pair(&empty[s]);
+              tc::commit_pair(&acc_full[b]);
+            } else {
+              tc::commit(&empty[s]);
+              tc::commit(&acc_full[b]);
+            }
           }
         }
         // Every MMA this thread issued has finished before TMEM can be freed.
-        tc::commit(mma_idle);
+        if (kPair)
+          tc::commit_pair(mma_idle);
+        else
+          tc::commit(mma_idle);
         mbar_wait_bounded(mma_idle, 0, abort_flag, p.err, kErrDrain);
       }
     } else if (warp == S::kEpi + 2) {
       // -------------------------------- scales ------------------------------
       int it = 0;
       for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-        const int m0 = tile % p.token_tiles * S::kTokens;
+        const int m0 = (tile % p.token_tiles * per_pair + pair_rank) * S::kTokens;
         const int n0 = tile / p.token_tiles * kTileOuts;
         const float* sx = p.x_scales + (m0 + lane) * p.xs_row;
         const float* sw = p.w_scales + (n0 / 128 + lane) * p.ws_row;
@@ -314,7 +359,12 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + col0;
     auto release = [&](uint64_t* bar) {  // the accumulator has been read
       tc::fence_before_sync();
-      if (lane == 0) mbar_arrive(bar);
+      if (lane == 0) {
+        if (kPair)
+          mbar_arrive_remote(cluster_address(bar, 0));
+        else
+          mbar_arrive(bar);
+      }
     };
     int it = 0;
     for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
@@ -380,7 +430,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
         }
       }
       if (!ok) break;
-      if (p.splits > 1) {
+      if (!kPair && p.splits > 1) {
         // One tile per CTA: its stages are free, every copy and MMA has finished.
         float* part = reinterpret_cast<float*>(stages) + col0 * kPartPitch + row;
 #pragma unroll
@@ -390,7 +440,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
           part[(2 * i + 1) * kPartPitch] = f.y;
         }
       } else if (TOKEN_ROWS) {
-        const int m = tile % p.token_tiles * kRows + row;
+        const int m = (tile % p.token_tiles * per_pair + pair_rank) * kRows + row;
         const int n0 = tile / p.token_tiles * COLS + col0;
         if (m < p.m && n0 < p.n) {
           T* out = reinterpret_cast<T*>(p.out) + static_cast<long long>(m) * p.out_stride + n0;
@@ -438,7 +488,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     }
   }
   __syncwarp();  // single-thread roles rejoin their warp
-  if (p.splits > 1) {
+  if (!kPair && p.splits > 1) {
     // Join: rank r adds the tokens [kTokens r / splits, ...) of all ranks, in rank
     // order; lanes take neighbouring outputs.
     cluster.sync();
@@ -463,9 +513,13 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
   // ---- teardown: every TMEM access is done, the MMA warp frees TMEM ----
   tc::fence_before_sync();
   __syncthreads();
+  if (kPair) cluster.sync();  // rank 0's MMAs read and write both CTAs' memory
   if (warp == S::kEpi + 1) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, S::kTmemCols);
+    if (kPair)
+      tc::tmem_dealloc_pair(tmem, S::kTmemCols);
+    else
+      tc::tmem_dealloc(tmem, S::kTmemCols);
   }
 }
 
@@ -492,7 +546,7 @@ int launch(const CUtensorMap& wmap, const CUtensorMap& xmap, const LinearParams&
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(S::kPair ? 2 : p.splits);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -508,20 +562,23 @@ int launch_any(const b200_fp8_linear_args* a, const void* x, const void* w, Line
   using S = Shape<COLS, TOKEN_ROWS>;
   const int slots = sms * S::kCtasPerSm;
   const int tile_outs = TOKEN_ROWS ? COLS : kRows;
-  p.token_tiles = static_cast<int>(ceil_div64(a->m, S::kTokens));
+  const int per_tile = S::kPair ? 2 : 1;
+  p.token_tiles = static_cast<int>(ceil_div64(a->m, S::kTokens * per_tile));
   const long long tiles = ceil_div64(a->n, tile_outs) * p.token_tiles;
   if (tiles > 0x7fffffffLL / kMaxSplits)
     return set_error(B200_ERR_UNSUPPORTED, "too many output tiles");
   p.tiles = static_cast<int>(tiles);
   // Splits of K that still fit the CTAs at once, each with two blocks or more.
-  p.splits = static_cast<int>(std::max<long long>(
-      1, std::min<long long>({kMaxSplits, slots / p.tiles, p.blocks / 2})));
-  const long long ctas = p.splits > 1 ? tiles * p.splits : std::min<long long>(tiles, slots);
+  p.splits = S::kPair ? 1
+                      : static_cast<int>(std::max<long long>(
+                            1, std::min<long long>({kMaxSplits, slots / tiles, p.blocks / 2})));
+  const long long ctas = p.splits > 1 ? tiles * p.splits
+                                      : std::min<long long>(tiles, slots / per_tile) * per_tile;
   const uint64_t wdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->n)};
   const uint64_t xdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->m)};
   const uint64_t wstride[1] = {static_cast<uint64_t>(a->w_stride)};
   const uint64_t xstride[1] = {static_cast<uint64_t>(a->x_stride)};
-  const uint32_t wbox[2] = {kBlock, static_cast<uint32_t>(tile_outs)};
+  const uint32_t wbox[2] = {kBlock, static_cast<uint32_t>(S::kPair ? S::kLoadCols : tile_outs)};
   const uint32_t xbox[2] = {kBlock, static_cast<uint32_t>(S::kTokens)};
   CUtensorMap wmap, xmap;
   int rc = encode_tensor_map_8b(w, 2, wdims, wstride, wbox, &wmap);
@@ -592,8 +649,8 @@ int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const flo
   if (a->m <= 32) return launch_any<32, false>(a, x, w, p, sms, stream);
   if (a->m <= 64) return launch_any<64, false>(a, x, w, p, sms, stream);
   if (a->m <= 128) return launch_any<128, false>(a, x, w, p, sms, stream);
-  // 256 columns halve what a tile reads of x, if their tiles still fill the SMs.
-  if (ceil_div64(a->m, kRows) * ceil_div64(a->n, 256) >= sms)
+  // Pairs, where their tiles fill the SMs.
+  if (ceil_div64(a->m, 2 * kRows) * ceil_div64(a->n, 256) >= sms / 2)
     return launch_any<256, true>(a, x, w, p, sms, stream);
   return launch_any<128, true>(a, x, w, p, sms, stream);
 }

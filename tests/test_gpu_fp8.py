@@ -124,7 +124,9 @@ def _close(got, value, size, blocks, dtype):
     (1, 1, 16), (1, 128, 128), (1, 6144, 4096), (2, 129, 144), (15, 200, 1024), (16, 127, 256),
     (17, 384, 112), (31, 1000, 2048), (33, 257, 4096), (64, 4096, 1024), (65, 300, 400),
     (100, 513, 14336), (128, 128, 640), (129, 130, 768), (200, 1000, 512), (256, 256, 256),
-    (257, 385, 1040), (700, 2049, 384), (1000, 7, 2048), (2048, 1024, 128)])
+    (257, 385, 1040), (700, 2049, 384), (1000, 7, 2048), (2048, 1024, 128),
+    # enough tiles for pairs of CTAs: ragged in every direction, one block and many
+    (2100, 2309, 272), (300, 9500, 1040), (4097, 1281, 16), (2560, 2048, 4096)])
 def test_product_against_64_bits(dtype, m, n, k):
     dtype = DTYPES[dtype]
     x = _normal((m, k), m + n + k, dtype, 2.0)
