@@ -310,11 +310,11 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
                 tc::mma_e4m3(d, da, db, idesc, k > 0);
             }
             if (kPair) {
-              tc::commit_pair(&empty[s]);
               tc::commit_pair(&acc_full[b]);
+              tc::commit_pair(&empty[s]);
             } else {
-              tc::commit(&empty[s]);
               tc::commit(&acc_full[b]);
+              tc::commit(&empty[s]);
             }
           }
         }
@@ -381,6 +381,10 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
         load_columns(base, va);
         // Meanwhile the scales: with tokens as rows, this row's.
         ok = warp_wait(&sc_full[r], (it / kScaleRing) & 1, abort_flag, p.err);
+        if (!ok) {
+          tc::wait_ld(va);
+          break;
+        }
         const float* sc = scales + r * S::kScales;
         const float sw = sc[S::kTokens + group];
         const float s1 = TOKEN_ROWS ? sc[row] * sw : sw;
