@@ -118,7 +118,8 @@ struct LinearParams {
   int blocks;  // of K
   int token_tiles;
   int tiles, splits;
-  int wide_stores;  // 32-byte stores of a token's outputs
+  int wide_stores;   // 32-byte stores of a token's outputs
+  int weight_first;  // the weight may be read ahead of griddepcontrol.wait
 };
 
 // d += a * b on two packed 32-bit values.
@@ -235,7 +236,10 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
   if (kPair) cluster.sync();  // the other CTA's barriers are in place, too
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Launched with programmatic stream serialization: nothing of the previous kernel
+  // may be read, and nothing that it reads be written, ahead of this wait.  Only the
+  // producer has something to do before it.
+  if (warp != S::kEpi) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   bool ok = true;
   const int row = (warp & 3) * 32 + lane;  // of the tile; TMEM lane
@@ -251,28 +255,49 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
       if (lane == 0) {
         tma_prefetch_desc(&wmap);
         tma_prefetch_desc(&xmap);
+        auto load_w = [&](int s, int kb, int n0) {
+          uint8_t* dst = stages + s * S::kStageBytes + (TOKEN_ROWS ? kRows * kBlock : 0);
+          if (kPair)
+            tma_load_2d_pair(dst, &wmap, cluster_address(&full[s], 0), kb * kBlock, n0);
+          else
+            tma_load_2d(dst, &wmap, &full[s], kb * kBlock, n0);
+        };
+        auto expect = [&](int s) {  // of a pair: both CTAs' bytes, on rank 0's barrier
+          if (!kPair)
+            mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+          else if (rank == 0)
+            mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);
+        };
+        // The weight does not come from the previous kernel where that is this call's
+        // quantiser, which has itself waited for everything before it: the first
+        // stages' weight tiles are loaded while it runs.
+        int early = 0;
+        if (p.weight_first && tile0 < p.tiles) {
+          const int n0 = tile0 / p.token_tiles * kTileOuts + (kPair ? rank * S::kLoadCols : 0);
+          for (; early < kStages && kb0 + early < kb1; ++early) {
+            expect(early);
+            load_w(early, kb0 + early, n0);
+          }
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         int it = 0;
         for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
           const int n0 = tile / p.token_tiles * kTileOuts + (kPair ? rank * S::kLoadCols : 0);
           const int m0 = (tile % p.token_tiles * per_pair + pair_rank) * S::kTokens;
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % kStages;
-            ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
-                                   kErrWaitEmpty);
-            if (!ok) break;
-            uint8_t* dst = stages + s * S::kStageBytes;
-            if (kPair) {  // both CTAs' bytes arrive on rank 0's barrier
-              const uint32_t bar = cluster_address(&full[s], 0);
-              if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);
-              tma_load_2d_pair(dst, &xmap, bar, kb * kBlock, m0);
-              tma_load_2d_pair(dst + kRows * kBlock, &wmap, bar, kb * kBlock, n0);
-            } else {
-              mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-              tma_load_2d(dst, TOKEN_ROWS ? &xmap : &wmap, &full[s], kb * kBlock,
-                          TOKEN_ROWS ? m0 : n0);
-              tma_load_2d(dst + kRows * kBlock, TOKEN_ROWS ? &wmap : &xmap, &full[s], kb * kBlock,
-                          TOKEN_ROWS ? n0 : m0);
+            if (it >= early) {
+              ok = mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, abort_flag, p.err,
+                                     kErrWaitEmpty);
+              if (!ok) break;
+              expect(s);
+              load_w(s, kb, n0);
             }
+            uint8_t* dst = stages + s * S::kStageBytes + (TOKEN_ROWS ? 0 : kRows * kBlock);
+            if (kPair)
+              tma_load_2d_pair(dst, &xmap, cluster_address(&full[s], 0), kb * kBlock, m0);
+            else
+              tma_load_2d(dst, &xmap, &full[s], kb * kBlock, m0);
           }
         }
         if (!kPair || rank == 0) drain_stages<kStages>(full, it, p.err);
@@ -505,8 +530,13 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
         const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n0 + o]) : 0.f;
         for (int t = S::kTokens * rank / p.splits; t < t1; ++t) {
           const float* at = part + (TOKEN_ROWS ? o * kPartPitch + t : t * kPartPitch + o);
-          float sum = 0.f;
-          for (int r = 0; r < p.splits; ++r) sum += *cluster.map_shared_rank(at, r);
+          float from[kMaxSplits], sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < kMaxSplits; ++r)  // every remote load in flight at once
+            from[r] = *cluster.map_shared_rank(at, min(r, p.splits - 1));
+#pragma unroll
+          for (int r = 0; r < kMaxSplits; ++r)
+            if (r < p.splits) sum += from[r];
           reinterpret_cast<T*>(p.out)[(m0 + t) * p.out_stride + n0 + o] =
               from_float<E>(sum + bias);
         }
@@ -637,6 +667,7 @@ int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const flo
   p.x_scales = x_scales;
   p.w_scales = w_scales;
   p.bias = bias;
+  p.weight_first = args->x_dtype != B200_E4M3;  // the previous kernel is the quantiser above
   p.out = out;
   p.err = error_word;
   p.m = static_cast<int>(a->m);

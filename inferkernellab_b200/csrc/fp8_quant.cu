@@ -69,6 +69,9 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantPara
   const long long col = block * 128LL + lane8 * 16;
   const bool live = row < p.rows && col < p.cols;  // cols % 16 == 0 here
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // The product that follows may begin to load its weight: it waits for this grid
+  // before it reads what this grid writes.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   uint4 a = {}, b = {};
   if (live) {
     const uint4* src = reinterpret_cast<const uint4*>(p.x + row * p.x_stride + col);
