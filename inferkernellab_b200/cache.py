@@ -37,11 +37,12 @@ class BlockAllocator:
     reuses freed ids last-freed-first, matching reference ``cache.py:17-64``;
     ``free`` validates the whole request before releasing anything.
 
-    Blocks carry a reference count (prefix sharing, ``prefix_cache.py``):
-    ``share`` adds a holder to allocated blocks and ``free`` drops one; a block
-    returns to the free stack when its last holder frees it.  A block with a
-    single holder behaves exactly as in the reference (same order, same owner
-    checks); the owner check is skipped for blocks that are shared.
+    Blocks carry a reference count (prefix sharing, ``prefix_cache.py``; forked
+    requests): ``share`` adds a holder to allocated blocks and ``free`` drops one;
+    a block returns to the free stack when its last holder frees it.  A block with
+    a single holder behaves exactly as in the reference (same order, same owner
+    checks); the owner check is skipped for blocks that are shared.  Holders that
+    ``share`` names take the block over, in order, when its owner frees it.
     """
 
     def __init__(self, num_blocks: int):
@@ -53,6 +54,7 @@ class BlockAllocator:
         self._in_use: set[int] = set()
         self._owner_of: dict[int, int] = {}
         self._refs: dict[int, int] = {}
+        self._next_owners: dict[int, list[int]] = {}  # named holders besides the owner
 
     @property
     def num_free_blocks(self) -> int:
@@ -90,20 +92,34 @@ class BlockAllocator:
             refs = self._refs.get(block, 1) - 1
             if refs > 0:
                 self._refs[block] = refs
+                self._drop_holder(block, owner)
                 continue
             self._refs.pop(block, None)
+            self._next_owners.pop(block, None)
             self._in_use.discard(block)
             self._owner_of.pop(block, None)
             self._stack.append(block)
 
-    def share(self, block_ids) -> None:
-        """Add one holder to each allocated block of ``block_ids``."""
+    def _drop_holder(self, block: int, owner: int | None) -> None:
+        """``owner`` has freed a block that others still hold."""
+        named = self._next_owners.get(block)
+        if owner is None or not named:
+            return
+        if self._owner_of.get(block) == owner:
+            self._owner_of[block] = named.pop(0)
+        elif owner in named:
+            named.remove(owner)
+
+    def share(self, block_ids, owner: int | None = None) -> None:
+        """Add one holder, ``owner`` if given, to each allocated block of ``block_ids``."""
         ids = tuple(block_ids)
         for block in ids:
             if not isinstance(block, int) or block not in self._in_use:
                 raise ValueError(f"block {block} is not allocated")
         for block in ids:
             self._refs[block] = self._refs.get(block, 1) + 1
+            if owner is not None:
+                self._next_owners.setdefault(block, []).append(owner)
 
     def ref_count(self, block_id: int) -> int:
         """Holders of ``block_id`` (0 when it is free)."""
@@ -144,6 +160,35 @@ class PagedKVCache:
 
     def release_request(self, block_table, request_id: int | None = None) -> None:
         self.allocator.free(block_table, owner=request_id)
+
+    def fork_request(self, block_table, num_tokens: int, request_ids) -> list[list[int]]:
+        """Block tables of forks of a request whose first ``num_tokens`` tokens are cached.
+
+        Each fork shares the full blocks; a last, partly filled block (which the
+        forks go on to write differently) is copied to a new one per fork, in every
+        layer, in one launch on the current stream.  All-or-nothing.
+        """
+        ids = list(request_ids)
+        if num_tokens <= 0:
+            raise ValueError("num_tokens must be positive")
+        full, rest = divmod(num_tokens, self.layout.block_size)
+        if len(block_table) < full + (rest > 0):
+            raise ValueError("block_table is shorter than num_tokens")
+        copies = len(ids) if rest else 0
+        if copies > self.allocator.num_free_blocks:
+            raise RuntimeError(f"out of KV blocks: requested={copies}, "
+                               f"free={self.allocator.num_free_blocks}")
+        shared = list(block_table[:full])
+        tables = []
+        for rid in ids:
+            self.allocator.share(shared, owner=rid)
+            tables.append(shared + (self.allocator.allocate(1, owner=rid) if rest else []))
+        if copies:
+            from .ops import copy_kv_pages
+
+            copy_kv_pages(self, [block_table[full]] * copies, [t[-1] for t in tables],
+                          tokens=[rest] * copies)
+        return tables
 
     def slot_mapping(self, block_table, start: int, length: int) -> torch.Tensor:
         """int64 physical slots of logical tokens ``start .. start+length-1``.

@@ -117,6 +117,18 @@ def main(argv=None) -> int:
                         "wall clock); default: the host prepares step N+1 while step N runs")
     p.add_argument("--unfused-decode", action="store_true",
                    help="rotary append and attention as two launches per layer (A/B check)")
+    p.add_argument("--projections", choices=("model", "fp8"), default="model",
+                   help="fp8: 8-bit weights and activations with block scales")
+    p.add_argument("--qk-norm", action="store_true",
+                   help="a norm on every query and key head of every layer")
+    p.add_argument("--sampler", choices=("torch", "device"), default="torch",
+                   help="device: one sampling launch per step for the whole batch")
+    p.add_argument("--temperature", type=float, default=0.0)
+    p.add_argument("--top-k", type=int, default=0)
+    p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=0.0)
+    p.add_argument("--samples-per-prompt", type=int, default=1, metavar="N",
+                   help="prefill every prompt once and fork it into N requests")
     p.add_argument("--trace-steps", default=None, metavar="A:B",
                    help="record a CUPTI kernel trace of decode steps A..B-1 (rank 0) and "
                         "print the per-kernel device time per step as a second JSON line")
@@ -148,9 +160,11 @@ def main(argv=None) -> int:
                                   max_position_embeddings=(args.max_prompt + args.shared_prefix
                                                            + args.max_new_tokens),
                                   rope_theta=args.rope_theta, seed=args.seed, device=device,
-                                  dtype=torch.bfloat16, init_on_device=True)
+                                  dtype=torch.bfloat16, init_on_device=True,
+                                  qk_norm=args.qk_norm)
         init_s = time.perf_counter() - t0
-        exchange = allgather_token_exchange(max_local=per) if world > 1 else None
+        exchange = (allgather_token_exchange(max_local=per * args.samples_per_prompt)
+                    if world > 1 else None)
         runner = LlamaPagedDecodeRunner(model, mine, max_new_tokens=args.max_new_tokens,
                                         block_size=args.block_size,
                                         max_num_batched_tokens=args.max_num_batched_tokens,
@@ -158,7 +172,11 @@ def main(argv=None) -> int:
                                         cuda_graph=not args.no_cuda_graph,
                                         prefix_caching=args.prefix_caching,
                                         sync_steps=args.sync_steps,
-                                        fused_decode=False if args.unfused_decode else "auto")
+                                        fused_decode=False if args.unfused_decode else "auto",
+                                        projections=args.projections, sampler=args.sampler,
+                                        temperature=args.temperature, top_k=args.top_k,
+                                        top_p=args.top_p, min_p=args.min_p,
+                                        samples_per_prompt=args.samples_per_prompt)
         trace = _StepTrace(runner, args.trace_steps) if (args.trace_steps and rank == 0) else None
         if world > 1:
             torch.distributed.barrier()
@@ -169,7 +187,8 @@ def main(argv=None) -> int:
         # the steady-state rate is taken over the remaining steps.
         steady = steps[1:] if len(steps) > 1 else steps
         decode_ms = sum(steady)
-        tokens_steady = float(len(mine) * len(steady))
+        requests = len(mine) * args.samples_per_prompt
+        tokens_steady = float(requests * len(steady))
         stats = torch.tensor([decode_ms, result.prefill_wall_ms, result.decode_p50_ms,
                               tokens_steady, float(steps[0]), sum(steps),
                               float(result.prefix_cached_tokens)],
@@ -183,7 +202,7 @@ def main(argv=None) -> int:
             g = torch.stack(gathered).cpu()
             decode_max = float(g[:, 0].max())
             tokens = float(g[:, 3].sum())
-            all_tokens = float(len(prompts) * args.max_new_tokens)
+            all_tokens = float(len(prompts) * args.samples_per_prompt * args.max_new_tokens)
             record = {
                 "metric": f"decode tok/s (config5 Llama-3-8B-shaped, {len(prompts)} requests)",
                 "value": round(tokens / (decode_max / 1e3), 1),
@@ -212,6 +231,11 @@ def main(argv=None) -> int:
                            "sync_each_step": args.sync_steps,
                            "fused_decode": "off" if args.unfused_decode else "auto"},
             }
+            chosen = {"projections": args.projections, "qk_norm": args.qk_norm,
+                      "sampler": args.sampler, "temperature": args.temperature,
+                      "top_k": args.top_k, "top_p": args.top_p, "min_p": args.min_p,
+                      "samples_per_prompt": args.samples_per_prompt}
+            record["config"] |= {k: v for k, v in chosen.items() if v != p.get_default(k)}
             print(json.dumps(record), flush=True)
             if trace is not None:
                 print(json.dumps(trace.summary()), flush=True)

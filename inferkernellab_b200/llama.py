@@ -34,6 +34,18 @@ summation order.  Attention-side work is on the sm_100a kernels:
   instead of re-launching ~35 kernels per layer from Python every step as the
   reference runner does.
 
+Beyond the reference's runner (all off by default):
+
+* layers whose attention has ``q_norm`` and ``k_norm`` (a norm on every query and
+  key head) run ``qk_norm_rope_append`` in place of the rotary append;
+* ``projections="fp8"`` quantises the packed projections, o_proj and down_proj once
+  (128 x 128 blocks) and runs them with ``fp8_linear``;
+* ``sampler="device"`` draws a step's tokens with one ``sample_tokens`` launch
+  (temperature, ``top_k``, ``top_p``, ``min_p``) from uniform numbers of one seeded
+  generator; ``"torch"`` is the reference's request-by-request sampling;
+* ``samples_per_prompt=n`` prefills a prompt once and forks it: the n requests share
+  its full KV pages and each gets a copy of the last, partly filled one.
+
 Multi-GPU: requests are partitioned over ranks by the caller; each rank runs its
 own runner (own block pool) and passes ``token_exchange`` -- e.g.
 ``allgather_token_exchange`` -- which all-gathers the sampled token ids of every
@@ -52,6 +64,7 @@ import torch
 
 from .cache import PagedKVCache
 from .decode import DeviceBlockTables, _percentile
+from .fp8 import fp8_linear, quantize_fp8_weight
 from .prefix_cache import PrefixCache
 from .ops import (
     add_rmsnorm,
@@ -59,10 +72,12 @@ from .ops import (
     paged_decode_attention,
     paged_decode_attention_append,
     paged_prefill_attention_varlen,
+    qk_norm_rope_append,
     rope_append_kv,
     silu_mul,
 )
 from .runtime import InferenceRuntime
+from .sampling import sample_tokens
 from .scheduler import InferenceRequest, TokenBudgetScheduler
 
 
@@ -123,7 +138,9 @@ class LlamaPagedDecodeRunner:
                  eos_token_ids: Sequence[int] | None = None,
                  token_exchange: TokenExchange | None = None, collect_logits: bool = True,
                  cuda_graph: bool = False, prefix_caching: bool = False,
-                 sync_steps: bool = True, fused_decode: bool | str = "auto"):
+                 sync_steps: bool = True, fused_decode: bool | str = "auto",
+                 sampler: str = "torch", top_k: int = 0, min_p: float = 0.0,
+                 projections: str = "model", samples_per_prompt: int = 1):
         if not prompts:
             raise ValueError("at least one prompt is required")
         if max_new_tokens <= 0:
@@ -139,11 +156,25 @@ class LlamaPagedDecodeRunner:
         if (not math.isfinite(temperature) or temperature < 0 or not math.isfinite(top_p)
                 or not 0 < top_p <= 1):
             raise ValueError("temperature must be non-negative and top_p must be in (0, 1]")
+        if sampler not in {"torch", "device"}:
+            raise ValueError("sampler must be torch or device")
+        if top_k < 0 or not 0 <= min_p <= 1:
+            raise ValueError("top_k must be non-negative and min_p must be in [0, 1]")
+        if sampler == "torch" and (top_k or min_p):
+            raise ValueError("top_k and min_p need sampler='device'")
+        if projections not in {"model", "fp8"}:
+            raise ValueError("projections must be model or fp8")
+        if samples_per_prompt <= 0:
+            raise ValueError("samples_per_prompt must be positive")
         self.model = model
         param = next(model.parameters())
         self.device, self.dtype = param.device, param.dtype
         if self.device.type != "cuda":
             raise ValueError("the b200 backend needs the model on a CUDA device")
+        # Request ids run over prompts, then samples; the first sample of a prompt is
+        # prefilled, the others fork from it.
+        prompts = [p for p in prompts for _ in range(samples_per_prompt)]
+        self.samples_per_prompt = samples_per_prompt
         self.prompts = tuple(tuple(int(t) for t in p) for p in prompts)
         if any(not p for p in self.prompts):
             raise ValueError("prompts must be non-empty")
@@ -153,6 +184,8 @@ class LlamaPagedDecodeRunner:
         self.backend, self.append_backend, self.prefill_mode = backend, append_backend, prefill_mode
         self.max_new_tokens = max_new_tokens
         self.temperature, self.top_p = temperature, top_p
+        self.sampler, self.top_k, self.min_p = sampler, top_k, min_p
+        self.projections = projections
         self.eos_token_ids = set(eos_token_ids or ())
         if any(t < 0 or t >= vocab for t in self.eos_token_ids):
             raise ValueError("EOS token id is outside the configured vocabulary")
@@ -199,22 +232,28 @@ class LlamaPagedDecodeRunner:
             decode_fn=self._decode, prefix_cache=self.prefix_cache)
         self.requests = [self.runtime.submit(rid, len(p), max_new_tokens,
                                              token_ids=p if prefix_caching else None)
-                         for rid, p in enumerate(self.prompts)]
+                         for rid, p in enumerate(self.prompts) if rid % samples_per_prompt == 0]
         width = max(1, max(-(-(n + max_new_tokens) // block_size) for n in self.prompt_lengths))
-        self.meta = DeviceBlockTables(len(self.requests), width, self.device)
+        self.meta = DeviceBlockTables(len(self.prompts), width, self.device)
         self._prompt_logits: dict[int, torch.Tensor] = {}
         self._next_logits: dict[int, torch.Tensor] = {}
         self._batch_logits: tuple[tuple[int, ...], torch.Tensor] | None = None
         self._decode_logits: list[torch.Tensor] = []
-        self._generated: dict[int, list[int]] = {r.request_id: [] for r in self.requests}
-        self._token_logprobs: dict[int, list[float]] = {r.request_id: [] for r in self.requests}
-        self._sampling_logprobs: dict[int, list[float]] = {r.request_id: [] for r in self.requests}
-        self._finish_reasons = {r.request_id: "length" for r in self.requests}
+        ids = range(len(self.prompts))
+        self._generated: dict[int, list[int]] = {rid: [] for rid in ids}
+        self._token_logprobs: dict[int, list[float]] = {rid: [] for rid in ids}
+        self._sampling_logprobs: dict[int, list[float]] = {rid: [] for rid in ids}
+        self._finish_reasons = {rid: "length" for rid in ids}
         self._generators = {}
-        for r in self.requests:
+        for rid in ids:
             gen = torch.Generator(device=self.device)
-            gen.manual_seed(seed + r.request_id)
-            self._generators[r.request_id] = gen
+            gen.manual_seed(seed + rid)
+            self._generators[rid] = gen
+        # sampler="device": one generator of uniform numbers, and each step's log
+        # probabilities, read back when the run has ended
+        self._uniforms = torch.Generator(device=self.device)
+        self._uniforms.manual_seed(seed)
+        self._device_logprobs: list[tuple[tuple[int, ...], torch.Tensor, torch.Tensor]] = []
         self._has_run = False
         self._pack_weights()
 
@@ -231,8 +270,26 @@ class LlamaPagedDecodeRunner:
         self._qkv, self._gate_up = [], []
         for layer in self.model.model.layers:
             attn, mlp = layer.self_attn, layer.mlp
-            self._qkv.append(_pack_linears((attn.q_proj, attn.k_proj, attn.v_proj)))
-            self._gate_up.append(_pack_linears((mlp.gate_proj, mlp.up_proj)))
+            self._qkv.append(self._projection(*_pack_linears((attn.q_proj, attn.k_proj,
+                                                              attn.v_proj))))
+            self._gate_up.append(self._projection(*_pack_linears((mlp.gate_proj, mlp.up_proj))))
+        if self.projections == "fp8":
+            layers = self.model.model.layers
+            self._o = [self._projection(m.weight, m.bias)
+                       for m in (layer.self_attn.o_proj for layer in layers)]
+            self._down = [self._projection(m.weight, m.bias)
+                          for m in (layer.mlp.down_proj for layer in layers)]
+        else:
+            self._o = [layer.self_attn.o_proj for layer in self.model.model.layers]
+            self._down = [layer.mlp.down_proj for layer in self.model.model.layers]
+        self._qk_norms = [_qk_norm_args(layer.self_attn) for layer in self.model.model.layers]
+
+    def _projection(self, weight: torch.Tensor, bias: torch.Tensor | None):
+        """``x -> x @ weight.T + bias`` in the runner's projection type."""
+        if self.projections == "fp8":
+            q, scales = quantize_fp8_weight(weight)
+            return lambda x: fp8_linear(x, q, scales, bias=bias)
+        return lambda x: torch.nn.functional.linear(x, weight, bias)
 
     def _forward(self, token_ids: torch.Tensor, positions: torch.Tensor, attend) -> torch.Tensor:
         """Shared layer loop on a flat token batch ``[N]``; returns the final-norm
@@ -253,21 +310,29 @@ class LlamaPagedDecodeRunner:
         kvd = self.num_kv_heads * self.head_dim
         normed, residual = add_rmsnorm(None, hidden, *_norm_args(layers[0].input_layernorm))
         for index, layer in enumerate(layers):
-            weight, bias = self._qkv[index]
-            qkv = torch.nn.functional.linear(normed, weight, bias)
+            qkv = self._qkv[index](normed)
             q = qkv[:, :qd].view(n, self.num_heads, self.head_dim)
             k = qkv[:, qd:qd + kvd].view(n, self.num_kv_heads, self.head_dim)
             v = qkv[:, qd + kvd:].view(n, self.num_kv_heads, self.head_dim)
             attended = attend(index, q, k, v, cos, sin)
-            out = layer.self_attn.o_proj(attended.reshape(n, qd))
+            out = self._o[index](attended.reshape(n, qd))
             normed, residual = add_rmsnorm(out, residual,
                                            *_norm_args(layer.post_attention_layernorm))
-            weight, bias = self._gate_up[index]
-            act = silu_mul(torch.nn.functional.linear(normed, weight, bias))
-            out = layer.mlp.down_proj(act)
+            act = silu_mul(self._gate_up[index](normed))
+            out = self._down[index](act)
             following = layers[index + 1].input_layernorm if index + 1 < len(layers) else inner.norm
             normed, residual = add_rmsnorm(out, residual, *_norm_args(following))
         return normed
+
+    def _rope_append(self, q, k, v, cos, sin, slots, layer: int) -> torch.Tensor:
+        """Rotated query of a layer, its keys and values appended; with the layer's norms
+        of queries and keys, if it has any, in the same launch."""
+        norms = self._qk_norms[layer]
+        if norms is None:
+            return rope_append_kv(q, k, v, cos, sin, self.cache, slots, layer=layer)
+        q_weight, k_weight, eps = norms
+        return qk_norm_rope_append(q, k, v, q_weight, k_weight, cos, sin, self.cache, slots,
+                                   layer=layer, eps=eps)
 
     def _decode_body(self, token_ids: torch.Tensor, positions: torch.Tensor,
                      tables: torch.Tensor) -> torch.Tensor:
@@ -285,8 +350,8 @@ class LlamaPagedDecodeRunner:
             fused = positions.shape[0] * self.num_kv_heads <= 2 * _decode_ctas(self.device)
 
         def attend(layer, q, k, v, cos, sin):
-            if not fused:
-                q = rope_append_kv(q, k, v, cos, sin, self.cache, slots, layer=layer)
+            if not fused or self._qk_norms[layer] is not None:
+                q = self._rope_append(q, k, v, cos, sin, slots, layer)
                 return paged_decode_attention(q, self.cache, tables, lens, layer=layer,
                                               validate_inputs=False)
             return paged_decode_attention_append(q, k, v, self.cache, tables, lens, slots,
@@ -318,7 +383,7 @@ class LlamaPagedDecodeRunner:
         pos = pos.to(self.device, non_blocking=True)
 
         def attend(layer, q, k, v, cos, sin):
-            q = rope_append_kv(q, k, v, cos, sin, self.cache, slots, layer=layer)
+            q = self._rope_append(q, k, v, cos, sin, slots, layer)
             return paged_prefill_attention_varlen(q, self.cache, tables, cu, meta[0], meta[1],
                                                   layer=layer)
 
@@ -329,8 +394,7 @@ class LlamaPagedDecodeRunner:
         hidden = self._forward_prefill_packed((request,), (start,), (end,))
         if end == len(self.prompts[request.request_id]):
             logits = self.model.lm_head(hidden[-1:])[0].detach()
-            self._prompt_logits[request.request_id] = logits
-            self._next_logits[request.request_id] = logits
+            self._prompt_done(request.request_id, logits)
 
     def _prefill_batch(self, requests, starts, ends) -> None:
         lengths = [int(e) - int(s) for s, e in zip(starts, ends)]
@@ -346,8 +410,18 @@ class LlamaPagedDecodeRunner:
         if last:
             logits = self.model.lm_head(hidden[torch.tensor(last, device=self.device)]).detach()
             for rid, row in zip(rows, logits):
-                self._prompt_logits[rid] = row
-                self._next_logits[rid] = row
+                self._prompt_done(rid, row)
+
+    def _prompt_done(self, request_id: int, logits: torch.Tensor) -> None:
+        """A prompt's last token has been computed: its other samples fork here."""
+        ids = range(request_id, request_id + self.samples_per_prompt)
+        for rid in ids:
+            self._prompt_logits[rid] = logits
+            self._next_logits[rid] = logits
+        if len(ids) > 1:
+            self.requests += self.runtime.fork(request_id, ids[1:])
+            self.requests.sort(key=lambda r: r.request_id)
+            self.runtime.scheduler.running.sort(key=lambda r: r.request_id)
 
     def _sample_token(self, logits: torch.Tensor, generator: torch.Generator):
         """Temperature / top-p sampling as the reference does (hf_benchmark.py:581-605)."""
@@ -388,7 +462,14 @@ class LlamaPagedDecodeRunner:
         if self.collect_logits:
             self._decode_logits.append(used.detach().float().cpu())
         sampled = None
-        if self.temperature == 0 and not self.eos_token_ids:
+        if self.sampler == "device":
+            uniforms = torch.rand(len(requests), generator=self._uniforms, device=self.device)
+            next_tokens, logprobs, sampling = sample_tokens(
+                used, uniforms, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p,
+                min_p=self.min_p)
+            self._device_logprobs.append((tuple(r.request_id for r in requests), logprobs,
+                                          sampling))
+        elif self.temperature == 0 and not self.eos_token_ids:
             next_tokens = used.argmax(dim=-1).to(torch.long)
         else:
             sampled = [self._sample_token(used[i], self._generators[r.request_id])
@@ -453,6 +534,10 @@ class LlamaPagedDecodeRunner:
                 started = time.perf_counter()
                 torch.cuda.synchronize(self.device)
                 decode_ms[-1] += (time.perf_counter() - started) * 1000
+        for ids, logprobs, sampling in self._device_logprobs:
+            for rid, policy, drawn in zip(ids, logprobs.tolist(), sampling.tolist()):
+                self._token_logprobs[rid].append(policy)
+                self._sampling_logprobs[rid].append(drawn)
         if self.prefix_cache is not None:
             self.prefix_cache.clear()  # the index holds one reference per cached block
         cache_released = self.cache.allocator.num_used_blocks == 0
@@ -569,17 +654,32 @@ def _norm_args(norm) -> tuple[torch.Tensor, float]:
     return norm.weight, float(eps)
 
 
+def _qk_norm_args(attention) -> tuple[torch.Tensor, torch.Tensor, float] | None:
+    """(q weight, k weight, eps) of an attention with a norm on every head, else None."""
+    q_norm, k_norm = getattr(attention, "q_norm", None), getattr(attention, "k_norm", None)
+    if q_norm is None and k_norm is None:
+        return None
+    if q_norm is None or k_norm is None:
+        raise ValueError("attention layers need both q_norm and k_norm, or neither")
+    (q_weight, eps), (k_weight, k_eps) = _norm_args(q_norm), _norm_args(k_norm)
+    if eps != k_eps:
+        raise ValueError("q_norm and k_norm must share one epsilon")
+    return q_weight, k_weight, eps
+
+
 def load_random_llama(*, vocab_size: int, hidden_size: int, intermediate_size: int,
                       num_layers: int, num_attention_heads: int, num_kv_heads: int,
                       max_position_embeddings: int, rope_theta: float, seed: int,
                       device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16,
-                      init_on_device: bool = False):
+                      init_on_device: bool = False, qk_norm: bool = False):
     """Random-init ``LlamaForCausalLM`` like the reference's ``_load_model`` (hf_benchmark.py:698-745).
 
     ``init_on_device=False`` reproduces the reference bit for bit (CPU float32
     init after ``torch.manual_seed(seed)``, then cast); ``True`` initialises on
     the GPU in ``dtype`` (same N(0, 0.02) scheme, different random stream),
-    which is the practical way to build an 8B-parameter model.
+    which is the practical way to build an 8B-parameter model.  ``qk_norm`` gives every
+    attention layer a ``q_norm`` and a ``k_norm`` (weights ~ N(1, 0.1)), which the
+    runner applies; the eager Transformers forward does not know them.
     """
     from transformers import LlamaConfig, LlamaForCausalLM
 
@@ -602,6 +702,16 @@ def load_random_llama(*, vocab_size: int, hidden_size: int, intermediate_size: i
         model = LlamaForCausalLM(config)
     model.config._attn_implementation = "eager"
     model = model.to(device=device, dtype=dtype).eval()
+    if qk_norm:
+        from transformers.models.llama.modeling_llama import LlamaRMSNorm
+
+        dim = int(getattr(config, "head_dim", None) or hidden_size // num_attention_heads)
+        gen = torch.Generator().manual_seed(seed)
+        for layer in model.model.layers:
+            for name in ("q_norm", "k_norm"):
+                norm = LlamaRMSNorm(dim, eps=config.rms_norm_eps)
+                norm.weight.data.copy_(1 + 0.1 * torch.randn(dim, generator=gen))
+                setattr(layer.self_attn, name, norm.to(device=device, dtype=dtype))
     for parameter in model.parameters():
         parameter.requires_grad_(False)
     return model

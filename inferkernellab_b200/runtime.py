@@ -83,6 +83,32 @@ class InferenceRuntime:
         self.scheduler.add(request)
         return request
 
+    def fork(self, request_id: int, new_ids) -> list[InferenceRequest]:
+        """Forks of a request whose prompt is cached: they continue from its tokens so far.
+
+        They share its full blocks and get copies of its last, partly filled one
+        (``PagedKVCache.fork_request``), and join the decode batch.
+        """
+        ids = [int(i) for i in new_ids]
+        if len(set(ids)) != len(ids) or any(i in self._requests for i in ids):
+            raise ValueError("duplicate request_id in a fork")
+        parent = self._requests.get(request_id)
+        if parent is None or parent.finished or parent.prompt_remaining or not parent.block_table:
+            raise ValueError("only a request with a cached prompt that has not finished can fork")
+        tokens = parent.prompt_tokens + parent.generated_tokens
+        short = len(ids) - self.cache.allocator.num_free_blocks
+        if short > 0 and tokens % self.cache.layout.block_size and self.prefix_cache is not None:
+            self.prefix_cache.evict(short)
+        forks = []
+        for rid, table in zip(ids, self.cache.fork_request(parent.block_table, tokens, ids)):
+            fork = InferenceRequest(rid, parent.prompt_tokens, parent.max_new_tokens,
+                                    generated_tokens=parent.generated_tokens,
+                                    cached_tokens=parent.cached_tokens, block_table=table)
+            self._requests[rid] = fork
+            self.scheduler.add_running(fork)
+            forks.append(fork)
+        return forks
+
     def _allocate(self, count: int, owner: int) -> list[int]:
         allocator = self.cache.allocator
         if self.prefix_cache is not None and count > allocator.num_free_blocks:

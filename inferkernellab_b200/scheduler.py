@@ -61,6 +61,13 @@ class TokenBudgetScheduler:
             raise ValueError("only waiting requests can be added")
         self.waiting.append(request)
 
+    def add_running(self, request: InferenceRequest) -> None:
+        """A request whose prompt is in the cache already (a fork): joins the decode batch."""
+        if request.status != "waiting" or request.prompt_remaining:
+            raise ValueError("only requests with a cached prompt can start decoding")
+        request.status = "running"
+        self.running.append(request)
+
     def _take_prefill(self) -> tuple[list[InferenceRequest], int]:
         batch: list[InferenceRequest] = []
         used = 0
