@@ -63,6 +63,7 @@ constexpr int kRows = 128;   // rows of a tile = MMA M
 constexpr int kBlock = 128;  // K per scale block = bytes of a swizzled row
 constexpr int kScaleRing = 8;
 constexpr int kMaxSplits = 8;
+constexpr int kManyBlocks = 64;  // of K, from which tokens as rows are worth a join
 constexpr int kPartPitch = kRows + 1;  // of the sums that a cluster joins: both ways conflict-free
 
 // TOKEN_ROWS: tokens are the tile's rows and outputs its columns; else the reverse.
@@ -170,6 +171,46 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
                                           uint32_t* err) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, err, kErrWaitFull));
+}
+
+// Adds the sums of a tile's `p.splits` <= RANKS CTAs and stores this rank's share of
+// its tokens.  Remote loads of RANKS x TOKENS values are in flight at once: a loop
+// over them pays their latency each time (8 splits, one token: 10 us).
+template <typename E, typename S, bool TOKEN_ROWS, int RANKS, int TOKENS>
+__device__ __forceinline__ void join(cg::cluster_group& cluster, const LinearParams& p,
+                                     const float* part, int rank, int m0, int n0) {
+  using T = typename E::T;
+  constexpr int kTileOuts = TOKEN_ROWS ? S::kCols * S::kGroups : kRows;
+  constexpr int kSlices = S::kThreads / kTileOuts;
+  const int o = threadIdx.x % kTileOuts, n = n0 + o;
+  const int t1 = min(S::kTokens * (rank + 1) / p.splits, p.m - m0);
+  if (n >= p.n) return;
+  const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+  for (int t0 = S::kTokens * rank / p.splits + threadIdx.x / kTileOuts; t0 < t1;
+       t0 += kSlices * TOKENS) {
+    float from[RANKS][TOKENS];
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) {
+      const float* there = cluster.map_shared_rank(part, min(r, p.splits - 1));
+#pragma unroll
+      for (int i = 0; i < TOKENS; ++i) {
+        const int t = t0 + i * kSlices;
+        from[r][i] = 0.f;
+        if (r < p.splits && t < t1)
+          from[r][i] = there[TOKEN_ROWS ? o * kPartPitch + t : t * kPartPitch + o];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+      const int t = t0 + i * kSlices;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < RANKS; ++r) sum += from[r][i];
+      if (t < t1)
+        reinterpret_cast<T*>(p.out)[static_cast<long long>(m0 + t) * p.out_stride + n] =
+            from_float<E>(sum + bias);
+    }
+  }
 }
 
 template <typename E, int COLS, bool TOKEN_ROWS>
@@ -311,28 +352,30 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
     } else if (warp == S::kEpi + 1) {
       // ------------------------------ MMA issuer ----------------------------
       if (lane == 0 && (!kPair || rank == 0)) {
+        // The issue of a block has to fit into the MMAs of the one before: descriptors
+        // of stage 0 to which a stage's and a K step's 16-byte units are added (the
+        // address field does not overflow), and counters instead of divisions.
         const uint32_t idesc = tc::idesc_e4m3(kPair ? 2 * kRows : kRows, COLS);
-        const uint32_t st0 = smem_u32(stages);
-        int it = 0;
+        const uint64_t rows0 = tc::sdesc_sw128(smem_u32(stages), 16, 1024);
+        const uint64_t cols0 = tc::sdesc_sw128(smem_u32(stages) + kRows * kBlock, 16, 1024);
+        int s = 0, b = 0;
+        uint32_t stage_phase = 0, buffer_phase = 1;
         for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
-          for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const int s = it % kStages, b = it % kBuffers;
-            ok = mbar_wait_bounded(&acc_empty[b], ((it / kBuffers) & 1) ^ 1, abort_flag, p.err,
-                                   kErrWaitEmpty) &&
-                 mbar_wait_bounded(&full[s], (it / kStages) & 1, abort_flag, p.err, kErrWaitFull);
+          for (int kb = kb0; kb < kb1; ++kb) {
+            ok = mbar_wait_bounded(&full[s], stage_phase, abort_flag, p.err, kErrWaitFull) &&
+                 mbar_wait_bounded(&acc_empty[b], buffer_phase, abort_flag, p.err,
+                                   kErrWaitEmpty);
             if (!ok) break;
             tc::fence_after_sync();
-            const uint32_t rows = st0 + s * S::kStageBytes;
-            const uint32_t cols = rows + kRows * kBlock;
+            const uint64_t da = rows0 + static_cast<uint32_t>(s) * (S::kStageBytes / 16);
+            const uint64_t db = cols0 + static_cast<uint32_t>(s) * (S::kStageBytes / 16);
             const uint32_t d = tmem + b * S::kBufferCols;
 #pragma unroll
             for (int k = 0; k < kBlock / 32; ++k) {
-              const uint64_t da = tc::sdesc_sw128(rows + k * 32, 16, 1024);
-              const uint64_t db = tc::sdesc_sw128(cols + k * 32, 16, 1024);
               if (kPair)
-                tc::mma_e4m3_pair(d, da, db, idesc, k > 0);
+                tc::mma_e4m3_pair(d, da + 2 * k, db + 2 * k, idesc, k > 0);
               else
-                tc::mma_e4m3(d, da, db, idesc, k > 0);
+                tc::mma_e4m3(d, da + 2 * k, db + 2 * k, idesc, k > 0);
             }
             if (kPair) {
               tc::commit_pair(&acc_full[b]);
@@ -340,6 +383,14 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
             } else {
               tc::commit(&acc_full[b]);
               tc::commit(&empty[s]);
+            }
+            if (++s == kStages) {
+              s = 0;
+              stage_phase ^= 1;
+            }
+            if (++b == kBuffers) {
+              b = 0;
+              buffer_phase ^= 1;
             }
           }
         }
@@ -519,28 +570,18 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
   __syncwarp();  // single-thread roles rejoin their warp
   if (!kPair && p.splits > 1) {
     // Join: rank r adds the tokens [kTokens r / splits, ...) of all ranks, in rank
-    // order; lanes take neighbouring outputs.
+    // order; neighbouring threads take neighbouring outputs.
     cluster.sync();
-    if (warp < S::kEpi && ok) {
-      const int n0 = tile0 / p.token_tiles * kTileOuts;
+    if (*abort_flag == 0) {
       const int m0 = tile0 % p.token_tiles * S::kTokens;
-      const int t1 = min(S::kTokens * (rank + 1) / p.splits, p.m - m0);
+      const int n0 = tile0 / p.token_tiles * kTileOuts;
       const float* part = reinterpret_cast<const float*>(stages);
-      for (int o = tid; o < kTileOuts && n0 + o < p.n; o += S::kEpi * 32) {
-        const float bias = p.bias ? to_float<E>(reinterpret_cast<const T*>(p.bias)[n0 + o]) : 0.f;
-        for (int t = S::kTokens * rank / p.splits; t < t1; ++t) {
-          const float* at = part + (TOKEN_ROWS ? o * kPartPitch + t : t * kPartPitch + o);
-          float from[kMaxSplits], sum = 0.f;
-#pragma unroll
-          for (int r = 0; r < kMaxSplits; ++r)  // every remote load in flight at once
-            from[r] = *cluster.map_shared_rank(at, min(r, p.splits - 1));
-#pragma unroll
-          for (int r = 0; r < kMaxSplits; ++r)
-            if (r < p.splits) sum += from[r];
-          reinterpret_cast<T*>(p.out)[(m0 + t) * p.out_stride + n0 + o] =
-              from_float<E>(sum + bias);
-        }
-      }
+      if (p.splits <= 2)
+        join<E, S, TOKEN_ROWS, 2, 8>(cluster, p, part, rank, m0, n0);
+      else if (p.splits <= 4)
+        join<E, S, TOKEN_ROWS, 4, 4>(cluster, p, part, rank, m0, n0);
+      else
+        join<E, S, TOKEN_ROWS, 8, 2>(cluster, p, part, rank, m0, n0);
     }
     cluster.sync();  // no CTA leaves while another may still read its sums
   }
@@ -602,10 +643,14 @@ int launch_any(const b200_fp8_linear_args* a, const void* x, const void* w, Line
   if (tiles > 0x7fffffffLL / kMaxSplits)
     return set_error(B200_ERR_UNSUPPORTED, "too many output tiles");
   p.tiles = static_cast<int>(tiles);
-  // Splits of K that still fit the CTAs at once, each with two blocks or more.
-  p.splits = S::kPair ? 1
-                      : static_cast<int>(std::max<long long>(
-                            1, std::min<long long>({kMaxSplits, slots / tiles, p.blocks / 2})));
+  // Splits of K that still fit the CTAs at once, each with two blocks or more.  With
+  // tokens as rows a join moves 64 KB a CTA and costs about 25 blocks' time (256
+  // tokens, 4096 outputs: 29.5 us split and 19.7 whole at 32 blocks, 47 and 54 us at
+  // 112), so that K is split from 64 blocks on.
+  p.splits = S::kPair || (TOKEN_ROWS && p.blocks < kManyBlocks)
+                 ? 1
+                 : static_cast<int>(std::max<long long>(
+                       1, std::min<long long>({kMaxSplits, slots / tiles, p.blocks / 2})));
   const long long ctas = p.splits > 1 ? tiles * p.splits
                                       : std::min<long long>(tiles, slots / per_tile) * per_tile;
   const uint64_t wdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->n)};
@@ -683,7 +728,12 @@ int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const flo
   if (a->m <= 16) return launch_any<16, false>(a, x, w, p, sms, stream);
   if (a->m <= 32) return launch_any<32, false>(a, x, w, p, sms, stream);
   if (a->m <= 64) return launch_any<64, false>(a, x, w, p, sms, stream);
-  if (a->m <= 128) return launch_any<128, false>(a, x, w, p, sms, stream);
+  // Up to 128 tokens the weight's rows as MMA rows still pay where a long K has to be
+  // split over few tiles (128 tokens, 4096 outputs, 112 blocks: 31 us against 44);
+  // else tokens as rows, whose scales cost nothing per column (28672 outputs, 32
+  // blocks: 41 us against 55; 6144 outputs: 20 against 35).
+  if (a->m <= 128 && p.blocks >= kManyBlocks && ceil_div64(a->n, kRows) * 2 <= sms)
+    return launch_any<128, false>(a, x, w, p, sms, stream);
   // Pairs, where their tiles fill the SMs.
   if (ceil_div64(a->m, 2 * kRows) * ceil_div64(a->n, 256) >= sms / 2)
     return launch_any<256, true>(a, x, w, p, sms, stream);
