@@ -226,6 +226,18 @@ def test_temperatures_at_the_ends_of_the_range():
     assert tokens.tolist() == [1] * 4
 
 
+@pytest.mark.parametrize("setting", SETTINGS)
+def test_tokens_do_not_depend_on_the_batch(setting):
+    """A batch gives a row fewer CTAs than a row by itself: the masses are whole, the token the same."""
+    logits, uniforms = _logits(300, 20011, torch.bfloat16, 12)
+    together = sample_tokens(logits, uniforms, **SETTINGS[setting])
+    for i in range(0, 300, 37):
+        alone = sample_tokens(logits[i:i + 1], uniforms[i:i + 1], **SETTINGS[setting])
+        assert torch.equal(alone[0], together[0][i:i + 1])
+        for a, b in zip(alone[1:], together[1:]):
+            assert torch.allclose(a, b[i:i + 1], rtol=0, atol=2.0 ** -20)  # sums in another order
+
+
 def test_distribution_of_many_draws():
     """Evenly spaced uniform numbers reproduce the kept probabilities to one draw in n."""
     n = 4096
