@@ -17,7 +17,8 @@
 // prefill batch and the launch at a decode step.  A row (one head of one token)
 // belongs to D / 16 neighbouring lanes, each with the 8 pairs it rotates in two
 // 16-byte vectors, so the sum of squares takes log2(D / 16) shuffles and no
-// shared memory.
+// shared memory.  Measured (32 / 8 heads of 128, bf16): 8191 tokens 39.6 us, 5.2 TB/s
+// (0.79 of the measured copy rate); one token 2.1 us.
 #include <algorithm>
 
 #include "../../include/b200_paged_attn.h"
@@ -318,8 +319,9 @@ cudaError_t launch(const QkNormParams& p, long long tokens, bool vec, int sms,
                    cudaStream_t stream) {
   const int lanes = vec ? p.head_dim / 16 : 32;
   // More than a token per SM: ROWS q rows per thread, for the bytes in flight and
-  // the factors formed once.  Fewer: a group of lanes per row, for the shortest
-  // way through.
+  // the factors formed once (4000 tokens: 21.6 us against 63; 160: 3.4 against 3.8).
+  // Fewer: a group of lanes per row, for the shortest way through (148 tokens: 2.4 us
+  // against 3.4; 8: 2.1 against 3.0).
   const bool many = vec && tokens > sms;
   const long long groups = many  ? ceil_div64(p.num_q_heads, kRowsAtOnce)
                            : vec ? p.num_q_heads + p.num_kv_heads
