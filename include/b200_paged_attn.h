@@ -430,7 +430,7 @@ B200_API int b200_sample_tokens(const b200_sample_args* args, const void* logits
  * No counterpart in the reference: additions of this library.
  *
  * Quantise: one fp32 scale per block_rows x 128 values (block_rows 1 for
- * activations, 128 for weights): scale = max |x| / 448, q = rn(x * (448 / max |x|));
+ * activations, 128 for weights): scale = max |x| / 448, q = rn(x * (448 * (1 / max |x|)));
  * a block whose largest magnitude is below 2^-100 becomes zeros with scale 0.
  * scales[row / block_rows, column / 128] at the given element strides.
  */

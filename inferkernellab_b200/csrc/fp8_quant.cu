@@ -3,10 +3,11 @@
 // (weights).
 //
 //   peak  = max |x| over the block (0 if below 2^-100)
-//   scale = peak / 448,   q = rn_e4m3(x * (448 / peak)),   x ~ q * scale
+//   scale = peak / 448,   q = rn_e4m3(x * (448 * (1 / peak))),   x ~ q * scale
 //
-// The peak lands on 448 exactly, so nothing saturates.  A block whose peak is
-// below 2^-100 is stored as zeros with scale 0: 448 / peak would leave the
+// every product and quotient rounded to 32 bits.  The peak lands on 448 (a unit in
+// the last place of 32 bits beside it at most), so nothing saturates.  A block whose
+// peak is below 2^-100 is stored as zeros with scale 0: 1 / peak would leave the
 // range of 32 bits.  A block with a NaN gets a NaN peak (the largest magnitude
 // is taken on the bit patterns, where NaN sorts above infinity), and one with
 // an infinity gets scale infinity; both come back as NaN, like the product of a
@@ -52,13 +53,13 @@ __device__ __forceinline__ float f32_of_bits(uint32_t bits) {
   return to_float<E>(t);
 }
 
-// scale and 448 / peak of a block from the bits of its largest magnitude.
+// scale and 448 * (1 / peak) of a block from the bits of its largest magnitude.
 template <typename E>
 __device__ __forceinline__ void block_scale(uint32_t peak_bits, float* scale, float* inverse) {
   float peak = f32_of_bits<E>(peak_bits);
   if (peak < kFp8Flush) peak = 0.f;
   *scale = __fdiv_rn(peak, kFp8Max);
-  *inverse = peak == 0.f ? 0.f : __fdiv_rn(kFp8Max, peak);
+  *inverse = peak == 0.f ? 0.f : __fmul_rn(__frcp_rn(peak), kFp8Max);
 }
 
 // grid.x = row tile * blocks + block: neighbouring CTAs read neighbouring columns.

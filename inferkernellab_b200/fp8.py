@@ -38,7 +38,7 @@ def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     128 columns.
 
     ``scales[m, b] = max |x[m, 128 b : 128 b + 128]| / 448``; ``q`` is e4m3 ``[M, K]``, the nearest
-    value of ``x * (448 / max)``, with rows on 16-byte boundaries, and ``scales`` float32
+    value of ``x * (448 * (1 / max))``, with rows on 16-byte boundaries, and ``scales`` float32
     ``[M, ceil(K / 128)]``, stored block by block (the order in which ``fp8_linear`` reads it).  A
     block whose largest magnitude is below 2**-100 becomes zeros; one that holds a NaN or an
     infinity stands for NaN.

@@ -33,8 +33,7 @@ def _quantized(x, block_rows):
     b = _blocks(x, block_rows)
     peak = b.abs().amax(dim=(1, 3))
     peak = torch.where(peak < 2.0 ** -100, 0.0, peak)
-    # one rounding: a scalar divided by a tensor would be its reciprocal times the scalar
-    inverse = torch.where(peak == 0, 0.0, torch.full_like(peak, 448.0) / peak)
+    inverse = torch.where(peak == 0, 0.0, peak.reciprocal() * 448.0)
     q = (b * inverse[:, None, :, None]).to(torch.float8_e4m3fn)
     q = q.reshape(b.shape[0] * block_rows, -1)[:x.shape[0], :x.shape[1]]
     return q, peak / 448.0

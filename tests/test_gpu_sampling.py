@@ -249,6 +249,14 @@ def test_distribution_of_many_draws():
     assert bool(((counts - p).abs() <= 1.5 / n).all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("setting", ["plain", "greedy", "top_p", "all"])
+def test_the_largest_vocabulary(dtype, setting):
+    logits, uniforms = _logits(2, 376832, DTYPES[dtype], 31)
+    args = dict(temperature=1.0, top_k=None, top_p=None, min_p=None) | SETTINGS[setting]
+    _check(logits, uniforms, sample_tokens(logits, uniforms, **args), **args)
+
+
 def test_no_rows_and_refusals():
     logits = torch.randn((0, 11), device="cuda")
     assert [v.shape for v in sample_tokens(logits, torch.empty(0, device="cuda"))] == [(0,)] * 3
