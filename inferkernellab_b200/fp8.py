@@ -123,7 +123,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
             x = x.contiguous()
         # the 8-bit rows, on 16-byte boundaries, and the scales, block by block
         nbytes = rows * (-(-cols // 16) * 16 + 4 * blocks)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        workspace = weight.new_empty(nbytes)  # one byte an element
     code = _DTYPE_CODE.get(dtype)
     if code is None:
         raise ValueError("the result must be float16 or bfloat16")
@@ -132,7 +132,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
             raise ValueError("bias must be [N] with the result's dtype and device")
         bias = bias if bias.is_contiguous() else bias.contiguous()
     if out is None:
-        out = torch.empty((rows, outs), dtype=dtype, device=weight.device)
+        out = weight.new_empty((rows, outs), dtype=dtype)
     elif (out.shape != (rows, outs) or out.dtype != dtype or out.get_device() != index
           or out.stride(1) != 1):
         raise ValueError("out must be [M, N] with the result's dtype, on the weight's device")

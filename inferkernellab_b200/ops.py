@@ -67,15 +67,15 @@ def _stream_ptr(device: torch.device) -> ctypes.c_void_p:
 def _cache_desc(cache) -> _lib.CacheDesc:
     layout = cache.layout
     k, v = cache.k, cache.v
-    if k.dtype not in _DTYPE_CODE:
+    code = _DTYPE_CODE.get(k.dtype)
+    if code is None:
         raise ValueError("the B200 kernels support float16 and bfloat16 caches")
     if not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("cache K/V storage must be contiguous")
-    if k.device.type != "cuda":
+    if k.get_device() < 0:
         raise ValueError("the cache must live on a CUDA device")
     return _lib.CacheDesc(k.data_ptr(), v.data_ptr(), layout.num_layers, layout.num_blocks,
-                          layout.block_size, layout.num_kv_heads, layout.head_dim,
-                          _DTYPE_CODE[k.dtype])
+                          layout.block_size, layout.num_kv_heads, layout.head_dim, code)
 
 
 # ----------------------------------------------------------------- workspace
@@ -137,6 +137,9 @@ class _ErrorWords:
 
     def get(self, device: torch.device) -> torch.Tensor:
         index = device.index if device.index is not None else torch.cuda.current_device()
+        word = self._words.get(index)  # set once, never replaced
+        if word is not None:
+            return word
         with self._lock:
             word = self._words.get(index)
             if word is None:
@@ -498,15 +501,6 @@ def rope_append_kv(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     return out
 
 
-def _last_contiguous(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
-    """``t`` with a contiguous last dimension, and its strides."""
-    strides = t.stride()
-    if strides[-1] != 1:
-        t = t.contiguous()
-        strides = t.stride()
-    return t, strides
-
-
 def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                         q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
                         sin: torch.Tensor, cache, slots: torch.Tensor, layer: int = 0, *,
@@ -557,14 +551,19 @@ def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
     if slots_code is None:
         raise ValueError("slots must use int32 or int64")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=dtype, device=query.device)
+        out = query.new_empty((tokens, heads, dim))
     elif (out.shape != query.shape or out.dtype != dtype or out.get_device() != index
           or out.stride(-1) != 1):
         raise ValueError("out must match query's shape, dtype and device")
     if tokens == 0:
         return out
-    (query, qs), (key, ks), (value, vs), (cos, cs), (sin, ss), (q_weight, _), (k_weight, _) = map(
-        _last_contiguous, (query, key, value, cos, sin, q_weight, k_weight))
+    qs, ks, vs, cs, ss = query.stride(), key.stride(), value.stride(), cos.stride(), sin.stride()
+    if not (qs[2] == ks[2] == vs[2] == cs[1] == ss[1] == q_weight.stride(0) == k_weight.stride(0)
+            == 1):
+        query, key, value, cos, sin, q_weight, k_weight = (
+            t if t.stride(-1) == 1 else t.contiguous()
+            for t in (query, key, value, cos, sin, q_weight, k_weight))
+        qs, ks, vs, cs, ss = (t.stride() for t in (query, key, value, cos, sin))
     if slots.ndim != 1 or slots.stride(0) != 1:
         slots = slots.reshape(-1).contiguous()
     os = out.stride()
@@ -659,7 +658,7 @@ def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor, *,
         raise ValueError("page_map must be a 1-D int32 tensor on the tables' device")
     rows, width = block_tables.shape
     if out is None:
-        out = torch.empty((rows, width), dtype=block_tables.dtype, device=block_tables.device)
+        out = block_tables.new_empty((rows, width))
     elif (out.shape != block_tables.shape or out.dtype != block_tables.dtype
           or out.get_device() != index or (width > 1 and out.stride(1) != 1)):
         raise ValueError("out must match block_tables, with contiguous rows")

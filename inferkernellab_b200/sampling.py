@@ -98,7 +98,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1
         m_ptr = min_p.data_ptr()
     else:
         m = _number(min_p, "min_p", 0.0, lambda v: 0.0 <= v <= 1.0)
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    tokens = uniforms.new_empty(rows, dtype=torch.int64)
     logprobs, sampling = torch.empty_like(uniforms), torch.empty_like(uniforms)
     args = _lib.SampleArgs(rows, row_stride, vocab, code, t, k, p, m)
     _lib.check(_lib.load().b200_sample_tokens(
