@@ -53,7 +53,8 @@ enum {
   B200_DEVERR_WAIT_FULL = 1,  /* a consumer gave up waiting for a TMA stage (bounded wait) */
   B200_DEVERR_WAIT_EMPTY = 2, /* a producer gave up waiting for a free stage               */
   B200_DEVERR_BAD_SLOT = 4,   /* append skipped a slot outside [0, num_blocks*block_size)  */
-  B200_DEVERR_BAD_BLOCK = 8,  /* a block-table entry outside [0, num_blocks) was masked    */
+  B200_DEVERR_BAD_BLOCK = 8,  /* a block-table entry or page id outside [0, num_blocks)    */
+                              /* was masked (attention) or skipped (copies, remaps)        */
   B200_DEVERR_DRAIN = 16      /* a producer gave up draining its copies after an abort     */
 };
 
@@ -440,7 +441,8 @@ B200_API int b200_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_
 
 /* out[m, n] = sum_b x_scales[m, b] w_scales[n / 128, b] sum_{k in block b} x[m, k] w[n, k]
  * (+ bias[n]), blocks of 128 columns, 32-bit sums, rounded once to the output type.
- * w [n, k] is e4m3 with rows on 16-byte boundaries (w_stride a multiple of 16); bias
+ * w [n, k] is e4m3 with rows on 16-byte boundaries (w_stride a multiple of 16) that do
+ * not overlap; bias
  * (NULL: none) and out have type dtype.  x [m, k] is
  *   e4m3 (x_dtype B200_E4M3) with x_scales, rows on 16-byte boundaries; or
  *   16-bit of type dtype (x_dtype = dtype), quantised first as by b200_quantize_fp8

@@ -26,7 +26,7 @@ enum DeviceError : uint32_t {
   kErrWaitFull = 1u,      // consumer gave up waiting for a TMA stage
   kErrWaitEmpty = 2u,     // producer gave up waiting for a free stage
   kErrBadSlot = 4u,       // append: slot outside [0, num_blocks*block_size)
-  kErrBadBlock = 8u,      // a block-table entry outside [0, num_blocks) was masked
+  kErrBadBlock = 8u,      // a block-table entry or page id outside [0, num_blocks) was masked
   kErrDrain = 16u,        // producer gave up draining its own copies at abort
 };
 

@@ -663,8 +663,10 @@ int launch_any(const b200_fp8_linear_args* a, const void* x, const void* w, Line
                                       : std::min<long long>(tiles, slots / per_tile) * per_tile;
   const uint64_t wdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->n)};
   const uint64_t xdims[2] = {static_cast<uint64_t>(a->k), static_cast<uint64_t>(a->m)};
-  const uint64_t wstride[1] = {static_cast<uint64_t>(a->w_stride)};
-  const uint64_t xstride[1] = {static_cast<uint64_t>(a->x_stride)};
+  // A single row has no stride of its own; a map's must hold the row.
+  const int64_t pitch = ceil_div64(a->k, 16) * 16;
+  const uint64_t wstride[1] = {static_cast<uint64_t>(std::max<int64_t>(a->w_stride, pitch))};
+  const uint64_t xstride[1] = {static_cast<uint64_t>(std::max<int64_t>(a->x_stride, pitch))};
   const uint32_t wbox[2] = {kBlock, static_cast<uint32_t>(S::kPair ? S::kLoadCols : tile_outs)};
   const uint32_t xbox[2] = {kBlock, static_cast<uint32_t>(S::kTokens)};
   CUtensorMap wmap, xmap;
@@ -695,6 +697,9 @@ int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const flo
     return set_error(B200_ERR_UNSUPPORTED, "sizes are limited to 2^31 - 256");
   if (a->w_stride % 16 != 0 || (a->x_dtype == B200_E4M3 && a->x_stride % 16 != 0))
     return set_error(B200_ERR_INVALID, "rows of x and weight must start on 16-byte boundaries");
+  if ((a->n > 1 && a->w_stride < a->k) ||
+      (a->x_dtype == B200_E4M3 && a->m > 1 && a->x_stride < a->k))
+    return set_error(B200_ERR_INVALID, "rows of x and weight must not overlap");
   if (a->m == 0) return B200_OK;
   if (!x || !w || !w_scales || !out || (a->x_dtype == B200_E4M3 && !x_scales))
     return set_error(B200_ERR_INVALID, "null tensor pointer");

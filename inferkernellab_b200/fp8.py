@@ -103,7 +103,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
         if (x_scales.shape != (rows, blocks) or x_scales.dtype != torch.float32
                 or x_scales.get_device() != index):
             raise ValueError("x_scales must be float32 [M, ceil(K / 128)] on x's device")
-        if x.stride(1) != 1 or x.stride(0) % 16 or x.data_ptr() % 16:
+        if x.stride(1) != 1 or x.stride(0) % 16 or x.stride(0) < cols or x.data_ptr() % 16:
             padded = _empty_fp8(rows, cols, x.device)
             padded.copy_(x)
             x = padded

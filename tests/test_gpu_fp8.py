@@ -158,6 +158,13 @@ def test_bias_out_strides_and_scale_layouts():
     odd.copy_(xq)
     assert torch.equal(fp8_linear(odd, wq, ws, x_scales=xs.contiguous()), plain)
     assert torch.equal(fp8_linear(xq, wq, ws.t().contiguous().t(), x_scales=xs), plain)
+    # one row given many times, in both types; a weight of one row
+    rows = fp8_linear(xq[:1].expand(5, k), wq, ws, x_scales=xs[:1].expand(5, -1))
+    assert torch.equal(rows, plain[:1].expand(5, n))
+    assert torch.equal(fp8_linear(x[:1].expand(5, k), wq, ws), plain[:1].expand(5, n))
+    assert torch.equal(fp8_linear(x, wq[:1], ws[:1]), plain[:, :1])
+    with pytest.raises(ValueError, match="overlap"):
+        fp8_linear(x, wq[:1].expand(7, k), ws[:1])
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):

@@ -92,6 +92,8 @@ def test_quantize_fp8():
     (dict(n=2 ** 31), UNSUPPORTED, "2^31"),
     (dict(w_stride=100), INVALID, "16-byte"),
     (dict(x_stride=100), INVALID, "16-byte"),
+    (dict(w_stride=112), INVALID, "overlap"),
+    (dict(m=2, x_stride=0), INVALID, "overlap"),
     (dict(m=0), OK, ""),
 ])
 def test_fp8_linear(args, want, match):
