@@ -114,6 +114,9 @@ struct Shape {
   static_assert(kPartPitch * COLS * 4 <= kStages * kStageBytes || kPair,
                 "the split sums reuse the stages");
   static_assert(kSmem <= 227 * 1024 / kCtasPerSm - 1024, "shared memory");
+  // Two pairs (of launches on two streams) that each held one SM's TMEM and waited for
+  // the other's would wait for good: a pair's CTA leaves no room for another on its SM.
+  static_assert(!kPair || 2 * kSmem > 227 * 1024, "one CTA of a pair per SM");
 };
 
 struct LinearParams {

@@ -191,6 +191,23 @@ def test_rows_are_independent(m):
     assert bool((zero == 0).all())
 
 
+def test_products_on_several_streams_at_once():
+    """Every kind of tile (few, many tokens, split K, pairs) beside every other."""
+    xs = [_normal((m, 1024), m, torch.bfloat16) for m in (2500, 1, 64, 700)]
+    wq, ws = _weights(2560, 1024, 21)
+    want = [fp8_linear(x, wq, ws) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for i, stream in enumerate(streams):
+        with torch.cuda.stream(stream):
+            got.append([fp8_linear(xs[(i + j) % 4], wq, ws) for j in range(4)])
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        assert all(torch.equal(out, want[(i + j) % 4]) for j, out in enumerate(outs))
+    assert check_device_errors() == 0
+
+
 def test_refusals():
     x = _normal((4, 256), 1, torch.bfloat16)
     wq, ws = _weights(130, 256, 2)
