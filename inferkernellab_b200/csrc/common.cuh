@@ -172,6 +172,17 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
       : "memory");
 }
 
+// The two halves of a cluster barrier, called by every thread of the cluster.  Another
+// CTA's shared memory may be touched once that CTA is known to run, which an arrival
+// at entry and a wait ahead of the first access show at no cost in between.  Relaxed:
+// no memory is handed over.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait;" ::: "memory");
+}
+
 // shared::cluster address of `p` in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
   uint32_t a;

@@ -35,7 +35,8 @@
 // list or are all equal, and the draw takes another pass over the slice.
 //
 // Bound: latency.  A row goes through three cluster barriers (m; sums and bounds; the
-// list), each 0.5 to 1 us, and the passes between them.  Measured (graph replay): one
+// list), each 0.5 to 1 us, and the passes between them; a fourth, that every CTA of the
+// cluster runs, ends while the first pass loads.  Measured (graph replay): one
 // row of 128256 bf16 logits with top_p 11.6 us, 64 rows with mixed settings 53 us (a
 // flat row that needs the exact search takes 37 us of it, any other 11 to 17), 256
 // rows of 128257 32-bit logits with top_k 105 us, 1.25 TB/s: two slices of 64 KB share
@@ -320,6 +321,7 @@ class Row {
     m = warp_max(m);
     if (lane == 0) s.red_f[warp] = m;
     __syncthreads();
+    cluster_wait();  // of the arrival at entry: every CTA runs, its shared memory may be written
     if (warp == 0) {
       m = warp_max(s.red_f[lane % kWarps]);
       if (lane < ranks) at(lane)->max_of[rank] = m;
@@ -1019,6 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   Row<L> row(p, s, reinterpret_cast<Vec<L>*>(smem + kSharedBytes), cluster);
   const int tid = row.tid, warp = row.warp, lane = row.lane, rank = row.rank;
   const long long b = blockIdx.x / row.ranks;
+  cluster_arrive_relaxed();  // Row::load waits for it
   if (tid < kCoarse) s.coarse_count[tid] = s.coarse_mass[tid] = 0;
   if (tid == 0) {
     s.listed[0] = s.listed[1] = s.local_listed = 0;

@@ -1,0 +1,37 @@
+"""Orders inside the kernels that no run can be relied on to show.
+
+Shared memory of another CTA of a cluster may be touched only once that CTA is known to run, and
+must not be given up while anything is still on its way into it.  A store that comes too early, or
+an arrival that comes too late, is nearly always harmless by luck; so the order is read here from
+the kernels' sources.
+"""
+
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parents[1] / "inferkernellab_b200" / "csrc"
+
+
+def _source(name):
+    """A source without its comments, white space as single blanks."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+    return re.sub(r"\s+", " ", text)
+
+
+def _in_order(text, *parts):
+    at = -1
+    for part in parts:
+        found = text.find(part, at + 1)
+        assert found >= 0, f"{part!r} is missing after position {at}"
+        at = found
+
+
+def test_sampler_waits_for_its_cluster_before_the_first_remote_store():
+    text = _source("sample.cu")
+    load = text[text.index("void load(const L* row)"):text.index("float argument(float l)")]
+    assert load.index("cluster_wait()") < load.index("at(lane)->")
+    kernel = text[text.index("sample_kernel(const SampleParams p)"):]
+    _in_order(kernel, "cluster_arrive_relaxed()", "griddepcontrol.wait", "row.load(logits)")
+    # nothing leaves, and nothing touches another CTA, between the arrival and the wait
+    before = kernel[:kernel.index("row.load(logits)")]
+    assert "return;" not in before and "row.at(" not in before
