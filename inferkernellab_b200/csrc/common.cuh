@@ -115,6 +115,21 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// Wait for the end of what this CTA has in flight, ahead of giving up memory that it
+// reads or writes.  Bounded, and not cut short by the abort flag: an abort is when
+// something may still be on its way.
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, uint32_t* err_word) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      if (err_word) atomicOr(err_word, kErrDrain);
+      return false;
+    }
+  }
+  return true;
+}
+
 // -------------------------------------------------------------------- TMA
 // Hint: bring the 128-byte line holding `ptr` into L2.  No value is read, so it
 // is safe before griddepcontrol.wait (a later write by the previous kernel goes

@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
           tc::commit_pair(mma_idle);
         else
           tc::commit(mma_idle);
-        mbar_wait_bounded(mma_idle, 0, abort_flag, p.err, kErrDrain);
+        mbar_drain(mma_idle, 0, p.err);
       }
     } else if (warp == S::kEpi + 2) {
       // -------------------------------- scales ------------------------------

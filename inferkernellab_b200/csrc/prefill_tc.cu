@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       }
       // Every MMA this thread issued has finished before TMEM can be freed.
       tc::commit(mma_idle);
-      mbar_wait_bounded(mma_idle, 0, abort_flag, p.err, kErrDrain);
+      mbar_drain(mma_idle, 0, p.err);
     }
   } else {
     // ------------------------------ softmax ------------------------------

@@ -35,3 +35,15 @@ def test_sampler_waits_for_its_cluster_before_the_first_remote_store():
     # nothing leaves, and nothing touches another CTA, between the arrival and the wait
     before = kernel[:kernel.index("row.load(logits)")]
     assert "return;" not in before and "row.at(" not in before
+
+
+def test_an_abort_does_not_cut_short_the_wait_for_mmas_in_flight():
+    """TMEM is freed after every MMA has ended, after an abort too: that wait must not look at the
+    abort flag, as the waits inside the pipelines do."""
+    for name in ("fp8_linear.cu", "prefill_tc.cu"):
+        text = _source(name)
+        assert "mbar_wait_bounded(mma_idle" not in text, name
+        _in_order(text, "commit(mma_idle)", "mbar_drain(mma_idle, 0, p.err)", "tmem_dealloc")
+    common = _source("common.cuh")
+    drain = common[common.index("bool mbar_drain("):]
+    assert "abort_flag" not in drain[:drain.index("return true; }")]
