@@ -352,7 +352,16 @@ __global__ void __launch_bounds__(Shape<COLS, TOKEN_ROWS>::kThreads,
               tma_load_2d(dst, &xmap, &full[s], kb * kBlock, m0);
           }
         }
-        if (!kPair || rank == 0) drain_stages<kStages>(full, it, p.err);
+        // Rank 0's commits arrive on both CTAs' barriers.  Rank 1 sees the last of them,
+        // the stages' releases and then mma_idle, before its shared memory is given up.
+        if (kPair && rank == 1) {
+          for (int i = it; ok && i < it + kStages; ++i)
+            ok = mbar_wait_bounded(&empty[i % kStages], ((i / kStages) & 1) ^ 1, abort_flag,
+                                   p.err, kErrWaitEmpty);
+          mbar_drain(mma_idle, 0, p.err);
+        } else {
+          drain_stages<kStages>(full, it, p.err);
+        }
         // After an abort, rank 1's copies have no barrier of its own to wait for: far
         // longer than any copy takes.
         if (kPair && !ok)

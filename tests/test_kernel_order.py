@@ -47,3 +47,15 @@ def test_an_abort_does_not_cut_short_the_wait_for_mmas_in_flight():
     common = _source("common.cuh")
     drain = common[common.index("bool mbar_drain("):]
     assert "abort_flag" not in drain[:drain.index("return true; }")]
+
+
+def test_both_ctas_of_a_pair_see_the_last_commits_before_they_leave():
+    """Rank 0's commits arrive on rank 1's barriers asynchronously, and a cluster barrier does not
+    wait for them: rank 1 has to, for the stages' releases and for the last commit."""
+    text = _source("fp8_linear.cu")
+    producer = text[text.index("int early = 0;"):text.index("sdesc_sw128(smem_u32(stages)")]
+    _in_order(producer, "if (kPair && rank == 1) {", "i < it + kStages",
+              "mbar_wait_bounded(&empty[i % kStages]", "mbar_drain(mma_idle, 0, p.err)",
+              "drain_stages<kStages>")
+    teardown = text[text.index("__syncwarp(); if (!kPair && p.splits > 1)"):]
+    _in_order(teardown, "if (kPair) cluster.sync();", "tmem_dealloc_pair")
