@@ -42,7 +42,9 @@ Beyond the reference's runner (all off by default):
   (128 x 128 blocks) and runs them with ``fp8_linear``;
 * ``sampler="device"`` draws a step's tokens with one ``sample_tokens`` launch
   (temperature, ``top_k``, ``top_p``, ``min_p``) from uniform numbers of one seeded
-  generator; ``"torch"`` is the reference's request-by-request sampling;
+  generator; a request whose logits leave nothing to draw (all NaN or -inf) ends with
+  the finish reason ``"error"``; ``"torch"`` is the reference's request-by-request
+  sampling;
 * ``samples_per_prompt=n`` prefills a prompt once and forks it: the n requests share
   its full KV pages and each gets a copy of the last, partly filled one.
 
@@ -482,6 +484,9 @@ class LlamaPagedDecodeRunner:
         host_tokens = self._host_tokens[:len(requests)]
         host_tokens.copy_(next_tokens, non_blocking=True)
         self._tokens_ready.record()
+        if self.sampler == "device":
+            # -1: a row with nothing to draw; no id of the embedding.  Its request ends below.
+            next_tokens = next_tokens.clamp(min=0)
         positions = [r.prompt_tokens + r.generated_tokens for r in requests]
         ids = [r.request_id for r in requests]
         if self.cuda_graph and ids == list(range(len(ids))):
@@ -495,6 +500,10 @@ class LlamaPagedDecodeRunner:
         tokens = host_tokens.tolist()
         for row, request in enumerate(requests):
             token = int(tokens[row])
+            if token < 0:
+                self._finish_reasons[request.request_id] = "error"
+                request.max_new_tokens = request.generated_tokens + 1
+                continue
             self._generated[request.request_id].append(token)
             if sampled is not None:
                 self._token_logprobs[request.request_id].append(float(sampled[row][1].item()))
@@ -536,6 +545,8 @@ class LlamaPagedDecodeRunner:
                 decode_ms[-1] += (time.perf_counter() - started) * 1000
         for ids, logprobs, sampling in self._device_logprobs:
             for rid, policy, drawn in zip(ids, logprobs.tolist(), sampling.tolist()):
+                if policy == -math.inf:  # nothing was drawn
+                    continue
                 self._token_logprobs[rid].append(policy)
                 self._sampling_logprobs[rid].append(drawn)
         if self.prefix_cache is not None:
@@ -544,7 +555,8 @@ class LlamaPagedDecodeRunner:
         if len(self._prompt_logits) != len(self.requests):
             raise RuntimeError("prefill did not produce one final logits tensor per request")
         generated = tuple(tuple(self._generated[r.request_id]) for r in self.requests)
-        if any(not t or len(t) > self.max_new_tokens for t in generated):
+        if any((not t and self._finish_reasons[r.request_id] != "error")
+               or len(t) > self.max_new_tokens for r, t in zip(self.requests, generated)):
             raise RuntimeError("decoder finished with an invalid generated sequence length")
         element = torch.tensor([], dtype=self.dtype).element_size()
         lay = self.cache.layout
