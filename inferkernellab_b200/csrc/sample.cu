@@ -1158,8 +1158,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 template <typename L>
 int launch(const SampleParams& p, long long rows, int ranks, cudaStream_t stream) {
   const size_t smem = kSharedBytes + static_cast<size_t>(p.slice) * sizeof(L);  // slice: whole vectors
-  const cudaError_t err = cudaFuncSetAttribute(
-      sample_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // The limit belongs to the function, not to the call: always the largest, so that
+  // calls of other host threads never lower it ahead of this launch.
+  const cudaError_t err =
+      cudaFuncSetAttribute(sample_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           kSharedBytes + kMaxSlice * static_cast<int>(sizeof(L)));
   if (err != cudaSuccess) return cuda_status(err, "sample_kernel shared memory");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
