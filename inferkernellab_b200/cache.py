@@ -42,7 +42,9 @@ class BlockAllocator:
     a block returns to the free stack when its last holder frees it.  A block with
     a single holder behaves exactly as in the reference (same order, same owner
     checks); the owner check is skipped for blocks that are shared.  Holders that
-    ``share`` names take the block over, in order, when its owner frees it.
+    ``share`` names take the block over, in order, when its owner frees it.  A free
+    that names nobody may be any holder's: those named before it may all free the
+    block after it.
     """
 
     def __init__(self, num_blocks: int):
@@ -86,7 +88,8 @@ class BlockAllocator:
             if block not in self._in_use:
                 raise ValueError(f"block {block} is not allocated")
             if (owner is not None and self._refs.get(block, 1) == 1
-                    and self._owner_of.get(block) != owner):
+                    and self._owner_of.get(block) != owner
+                    and owner not in self._next_owners.get(block, ())):
                 raise ValueError(f"block {block} is not owned by request {owner}")
         for block in ids:
             refs = self._refs.get(block, 1) - 1

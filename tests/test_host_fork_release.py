@@ -1,0 +1,36 @@
+"""Forks released in any order, with and without naming who releases, and forks that fail."""
+
+import itertools
+
+import pytest
+
+from inferkernellab_b200 import BlockAllocator, PagedKVCache
+
+
+@pytest.mark.parametrize("unnamed", [u for n in range(4) for u in itertools.combinations((1, 2, 3), n)])
+@pytest.mark.parametrize("order", list(itertools.permutations((1, 2, 3))))
+def test_forks_release_in_any_order_named_or_not(order, unnamed):
+    cache = PagedKVCache(8, 4, 2, 16, device="cpu")
+    table = cache.allocate_request(1, 8)
+    tables = {1: table} | dict(zip((2, 3), cache.fork_request(table, 8, [2, 3])))
+    for i, rid in enumerate(order):
+        assert [cache.allocator.ref_count(b) for b in table] == [3 - i] * 2
+        cache.release_request(tables[rid], None if rid in unnamed else rid)
+    assert cache.allocator.num_used_blocks == 0
+    with pytest.raises(ValueError, match="not allocated"):
+        cache.release_request(table, 1)
+
+
+def test_a_named_release_is_still_checked():
+    a = BlockAllocator(4)
+    blocks = a.allocate(1, owner=1)
+    a.share(blocks, owner=2)
+    a.free(blocks)  # 1 or 2: who is left is not known
+    with pytest.raises(ValueError, match="not owned"):
+        a.free(blocks, owner=3)
+    a.free(blocks, owner=2)
+    blocks = a.allocate(1, owner=4)  # the same block: its holders of before are forgotten
+    with pytest.raises(ValueError, match="not owned"):
+        a.free(blocks, owner=2)
+    a.free(blocks, owner=4)
+    assert a.num_free_blocks == 4
