@@ -189,8 +189,13 @@ class PagedKVCache:
         if copies:
             from .ops import copy_kv_pages
 
-            copy_kv_pages(self, [block_table[full]] * copies, [t[-1] for t in tables],
-                          tokens=[rest] * copies)
+            try:
+                copy_kv_pages(self, [block_table[full]] * copies, [t[-1] for t in tables],
+                              tokens=[rest] * copies)
+            except BaseException:
+                for rid, table in zip(reversed(ids), reversed(tables)):
+                    self.allocator.free(table, owner=rid)
+                raise
         return tables
 
     def slot_mapping(self, block_table, start: int, length: int) -> torch.Tensor:

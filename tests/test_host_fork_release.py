@@ -34,3 +34,21 @@ def test_a_named_release_is_still_checked():
         a.free(blocks, owner=2)
     a.free(blocks, owner=4)
     assert a.num_free_blocks == 4
+
+
+def test_a_fork_whose_copy_fails_leaves_nothing_behind():
+    cache = PagedKVCache(8, 4, 2, 16, device="cpu")  # the page copy needs a CUDA cache
+    table = cache.allocate_request(1, 6)
+    expected = PagedKVCache(8, 4, 2, 16, device="cpu")
+    expected.allocate_request(1, 6)
+    for _ in range(3):
+        with pytest.raises(ValueError, match="CUDA"):
+            cache.fork_request(table, 6, [2, 3])
+    assert [cache.allocator.ref_count(b) for b in table] == [1, 1]
+    assert [cache.allocator.owner(b) for b in table] == [1, 1]
+    assert cache.allocator.num_used_blocks == 2
+    with pytest.raises(ValueError, match="not owned"):
+        cache.release_request(table, 2)  # a holder of the failed fork only
+    # what is handed out next is what it would have been
+    assert cache.allocator.allocate(6) == expected.allocator.allocate(6)
+    cache.release_request(table, 1)
