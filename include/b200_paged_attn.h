@@ -348,7 +348,8 @@ B200_API int b200_build_slot_mapping(const void* block_tables, int32_t table_dty
  *     query_out  = rope(n(query, q_weight)),  K[layer, slot] = rope(n(key, k_weight)),
  *     V[layer, slot] = value
  * All arithmetic in 32 bits, one rounding at the end.  cos/sin hold one row of
- * rotary_dim entries per token.  Any strides; last dimensions contiguous.
+ * rotary_dim entries per token.  Any strides; last dimensions contiguous; rows of
+ * query_out must not overlap.
  * Negative slots are skipped (q is still written); a slot past the pool sets
  * B200_DEVERR_BAD_SLOT.
  */
@@ -387,7 +388,8 @@ B200_API int b200_copy_kv_pages(const b200_cache_desc* cache, const void* src, c
 
 /* Rewrite block tables to new page ids: out[r, c] = page_map[tables[r, c]], page_map
  * int32 [num_blocks].  Negative entries (unused columns) stay; an entry past the
- * pool stays and sets B200_DEVERR_BAD_BLOCK.  out may be tables itself.
+ * pool stays and sets B200_DEVERR_BAD_BLOCK.  out may be tables itself; its rows must
+ * not overlap.
  */
 B200_API int b200_remap_block_tables(const void* tables, int32_t table_dtype, int64_t table_stride,
                             int64_t num_rows, int32_t table_width, const int32_t* page_map,
@@ -441,9 +443,9 @@ B200_API int b200_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_
 
 /* out[m, n] = sum_b x_scales[m, b] w_scales[n / 128, b] sum_{k in block b} x[m, k] w[n, k]
  * (+ bias[n]), blocks of 128 columns, 32-bit sums, rounded once to the output type.
- * w [n, k] is e4m3 with rows on 16-byte boundaries (w_stride a multiple of 16) that do
- * not overlap; bias
- * (NULL: none) and out have type dtype.  x [m, k] is
+ * w [n, k] is e4m3 with rows on 16-byte boundaries (w_stride a multiple of 16).  Rows of
+ * w, of an e4m3 x and of out must not overlap.  bias (NULL: none) and out have type
+ * dtype.  x [m, k] is
  *   e4m3 (x_dtype B200_E4M3) with x_scales, rows on 16-byte boundaries; or
  *   16-bit of type dtype (x_dtype = dtype), quantised first as by b200_quantize_fp8
  *   with block_rows 1, into `workspace`: m * (k rounded up to 16 + 4 * ceil(k / 128))

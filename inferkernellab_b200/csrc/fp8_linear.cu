@@ -712,6 +712,8 @@ int launch_fp8_linear(const b200_fp8_linear_args* args, const void* x, const flo
   if ((a->n > 1 && a->w_stride < a->k) ||
       (a->x_dtype == B200_E4M3 && a->m > 1 && a->x_stride < a->k))
     return set_error(B200_ERR_INVALID, "rows of x and weight must not overlap");
+  if (a->m > 1 && a->out_stride < a->n)
+    return set_error(B200_ERR_INVALID, "rows of out must not overlap");
   if (a->m == 0) return B200_OK;
   if (!x || !w || !w_scales || !out || (a->x_dtype == B200_E4M3 && !x_scales))
     return set_error(B200_ERR_INVALID, "null tensor pointer");

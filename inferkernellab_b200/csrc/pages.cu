@@ -155,6 +155,8 @@ int launch_remap_block_tables(const void* tables, int32_t table_dtype, int64_t t
     return set_error(B200_ERR_INVALID, "table or pool size out of range");
   if (num_rows == 0 || table_width == 0) return B200_OK;
   if (!tables || !page_map || !out) return set_error(B200_ERR_INVALID, "null tensor pointer");
+  if (num_rows > 1 && out_stride < table_width)
+    return set_error(B200_ERR_INVALID, "rows of out must not overlap");
   RemapParams p;
   p.tables = tables;
   p.page_map = page_map;

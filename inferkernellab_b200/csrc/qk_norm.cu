@@ -20,6 +20,7 @@
 // shared memory.  Measured (32 / 8 heads of 128, bf16): 8191 tokens 39.6 us, 5.2 TB/s
 // (0.79 of the measured copy rate); one token 2.1 us.
 #include <algorithm>
+#include <cstdint>
 
 #include "../../include/b200_paged_attn.h"
 #include "common.cuh"
@@ -303,6 +304,19 @@ __global__ void __launch_bounds__(1024) qk_norm_any_kernel(const QkNormParams p)
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether tokens x heads rows of `dim` elements share memory, unless one stride's
+// steps clear the extent of the other's.
+bool rows_overlap(int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride,
+                  int64_t dim) {
+  if (tokens == 1) token_stride = INT64_MAX;
+  if (heads == 1) head_stride = INT64_MAX;
+  const bool heads_inside = head_stride <= token_stride;
+  const int64_t inner = heads_inside ? head_stride : token_stride;
+  const int64_t outer = heads_inside ? token_stride : head_stride;
+  const int64_t count = heads_inside ? heads : tokens;
+  return inner < dim || (outer != INT64_MAX && outer < inner * (count - 1) + dim);
+}
+
 template <typename E, int ROWS>
 void (*vec_kernel(int lanes))(QkNormParams) {
   switch (lanes) {
@@ -364,6 +378,9 @@ int launch_qk_norm_rope_append(const b200_cache_desc* c, const b200_qk_norm_args
   if (!query || !key || !value || !q_weight || !k_weight || !cos || !sin || !slots ||
       !query_out || !c->k_cache || !c->v_cache)
     return set_error(B200_ERR_INVALID, "null tensor pointer");
+  if (rows_overlap(a->num_tokens, a->q_out_stride_token, a->num_q_heads, a->q_out_stride_head,
+                   c->head_dim))
+    return set_error(B200_ERR_INVALID, "rows of query_out must not overlap");
   QkNormParams p;
   p.q = static_cast<const uint8_t*>(query);
   p.k = static_cast<const uint8_t*>(key);

@@ -136,6 +136,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     elif (out.shape != (rows, outs) or out.dtype != dtype or out.get_device() != index
           or out.stride(1) != 1):
         raise ValueError("out must be [M, N] with the result's dtype, on the weight's device")
+    elif rows > 1 and out.stride(0) < outs:
+        raise ValueError("rows of out must not overlap")
     ws_row, ws_block = weight_scales.stride()
     args = _lib.Fp8LinearArgs(rows, outs, cols, x.stride(0), w_stride, out.stride(0), xs_row,
                               xs_block, ws_row, ws_block, code, x_code)

@@ -78,6 +78,18 @@ def _cache_desc(cache) -> _lib.CacheDesc:
                           layout.block_size, layout.num_kv_heads, layout.head_dim, code)
 
 
+def _rows_overlap(out: torch.Tensor) -> bool:
+    """Whether rows (the last dimension, contiguous) of an output share memory, in an order in
+    which one dimension's steps clear the other's extent, as every view of whole rows has."""
+    extent = out.shape[-1]
+    for stride, size in sorted(zip(out.stride()[:-1], out.shape[:-1])):
+        if size > 1:
+            if stride < extent:
+                return True
+            extent += stride * (size - 1)
+    return False
+
+
 # ----------------------------------------------------------------- workspace
 
 class _Workspaces:
@@ -555,6 +567,8 @@ def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
     elif (out.shape != query.shape or out.dtype != dtype or out.get_device() != index
           or out.stride(-1) != 1):
         raise ValueError("out must match query's shape, dtype and device")
+    elif _rows_overlap(out):
+        raise ValueError("rows of out must not overlap")
     if tokens == 0:
         return out
     qs, ks, vs, cs, ss = query.stride(), key.stride(), value.stride(), cos.stride(), sin.stride()
@@ -662,6 +676,8 @@ def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor, *,
     elif (out.shape != block_tables.shape or out.dtype != block_tables.dtype
           or out.get_device() != index or (width > 1 and out.stride(1) != 1)):
         raise ValueError("out must match block_tables, with contiguous rows")
+    elif _rows_overlap(out):
+        raise ValueError("rows of out must not overlap")
     if block_tables.stride(1) != 1:
         block_tables = block_tables.contiguous()
     page_map = page_map.contiguous()
