@@ -24,6 +24,8 @@ def _number(value, name: str, off, check):
     """A setting given as a number (``None``: off), checked."""
     if value is None:
         return off
+    if isinstance(off, int) and not isinstance(value, int) and not float(value).is_integer():
+        raise ValueError(f"{name} must be a whole number: {value}")
     value = type(off)(value)
     if not check(value):
         raise ValueError(f"{name} is out of range: {value}")
