@@ -85,6 +85,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1
         t_ptr = temperature.data_ptr()
     else:
         t = _number(temperature, "temperature", 1.0, lambda v: 0.0 <= v < math.inf)
+        if t > 0.0:
+            t = max(t, 2.0 ** -149)  # positive in 32 bits, too
     if isinstance(top_k, torch.Tensor):
         top_k = _per_row(top_k, "top_k", uniforms, torch.int32)
         k_ptr = top_k.data_ptr()

@@ -45,3 +45,15 @@ def test_host_threads_with_rows_of_different_sizes():
     assert not refused, (len(refused), refused[0])
     for _, _, want, token, *_ in jobs:
         assert torch.equal(token, want)
+
+
+def test_a_temperature_below_32_bits_is_not_greedy():
+    """1e-50 is no 32-bit number, but it is positive: equal largest logits are drawn from, and the
+    log-probabilities are those of that temperature, not of 1."""
+    logits = torch.tensor([[1.0, 2.0, 2.0, 0.0]] * 2, device="cuda")
+    uniforms = torch.tensor([0.1, 0.6], device="cuda")
+    tokens, logprobs, sampling = sample_tokens(logits, uniforms, temperature=1e-50)
+    assert tokens.tolist() == [1, 2]
+    half = torch.full_like(uniforms, 0.5)
+    assert torch.allclose(logprobs.exp(), half) and torch.allclose(sampling.exp(), half)
+    assert sample_tokens(logits, uniforms, temperature=0.0)[0].tolist() == [1, 1]
