@@ -599,10 +599,11 @@ def copy_kv_pages(cache, src, dst, *, tokens=None) -> None:
 
     ``tokens[i]`` limits pair ``i`` to its page's first tokens (a forked request's last, partly
     filled page); by default whole pages are copied.  ``src``, ``dst`` and ``tokens`` are lists, or
-    int32/int64 tensors of one dtype on the cache's device.  Lists are checked: valid ids, no page
-    the destination of two pairs or a destination and a source.  Device tensors are not read on the
-    host: a negative id skips its pair, an id past the pool skips it and sets the device error word,
-    and pages that overlap as above end up with either content.
+    int32/int64 tensors of one dtype on the cache's device.  Lists are checked, each by itself where
+    tensors stand beside it: valid ids, no page the destination of two pairs or a destination and a
+    source.  Device tensors are not read on the host: a negative id skips its pair, an id past the
+    pool skips it and sets the device error word, and pages that overlap as above end up with either
+    content.
     """
     device = cache.k.device
     if device.type != "cuda":
@@ -633,12 +634,15 @@ def _page_lists(layout, device, src, dst, tokens):
     """``copy_kv_pages`` arguments of which some are Python lists, checked, as device tensors."""
     given = [src, dst] if tokens is None else [src, dst, tokens]
     listed = [isinstance(v, (list, tuple)) for v in given]
-    if listed[0] and listed[1]:
-        if any(not 0 <= b < layout.num_blocks for b in (*src, *dst)):
-            raise ValueError("src/dst contain an invalid physical block id")
-        if len(set(dst)) != len(dst) or set(dst) & set(src):
-            raise ValueError("a page may be the destination of one copy only, and of none that "
-                             "reads it")
+    if any(not isinstance(v, int) and int(v) != v
+           for values, is_list in zip(given, listed) if is_list for v in values):
+        raise ValueError("src, dst and tokens must hold whole numbers")
+    pages = [b for values, is_list in zip((src, dst), listed) if is_list for b in values]
+    if any(not 0 <= b < layout.num_blocks for b in pages):
+        raise ValueError("src/dst contain an invalid physical block id")
+    if listed[1] and (len(set(dst)) != len(dst) or (listed[0] and set(dst) & set(src))):
+        raise ValueError("a page may be the destination of one copy only, and of none that "
+                         "reads it")
     if tokens is not None and listed[2] and any(not 0 <= n <= layout.block_size for n in tokens):
         raise ValueError("tokens must lie in [0, block_size]")
     if all(listed):  # one copy to the device
