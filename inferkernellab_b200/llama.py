@@ -42,7 +42,7 @@ Beyond the reference's runner (all off by default):
   (128 x 128 blocks) and runs them with ``fp8_linear``;
 * ``sampler="device"`` draws a step's tokens with one ``sample_tokens`` launch
   (temperature, ``top_k``, ``top_p``, ``min_p``) from uniform numbers of one seeded
-  generator; a request whose logits leave nothing to draw (all NaN or -inf) ends with
+  generator, one per request and step whoever has ended; a request whose logits leave nothing to draw (all NaN or -inf) ends with
   the finish reason ``"error"``; ``"torch"`` is the reference's request-by-request
   sampling;
 * ``samples_per_prompt=n`` prefills a prompt once and forks it: the n requests share
@@ -465,7 +465,12 @@ class LlamaPagedDecodeRunner:
             self._decode_logits.append(used.detach().float().cpu())
         sampled = None
         if self.sampler == "device":
-            uniforms = torch.rand(len(requests), generator=self._uniforms, device=self.device)
+            # A number for every request, ended or not: what one draws does not depend on
+            # which others are left.
+            uniforms = torch.rand(len(self.prompts), generator=self._uniforms, device=self.device)
+            if len(requests) < len(self.prompts):
+                rows = torch.tensor([r.request_id for r in requests])
+                uniforms = uniforms[rows.to(self.device, non_blocking=True)]
             next_tokens, logprobs, sampling = sample_tokens(
                 used, uniforms, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p,
                 min_p=self.min_p)

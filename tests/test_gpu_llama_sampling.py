@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from inferkernellab_b200 import check_device_errors
+from inferkernellab_b200 import check_device_errors, llama, sample_tokens
 from inferkernellab_b200.llama import LlamaPagedDecodeRunner, load_random_llama
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +61,39 @@ def test_no_request_has_anything_to_draw():
     got = runner.run()
     assert got.generated_tokens == ((), (), ()) and got.finish_reasons == ("error",) * 3
     assert got.cache_released
+
+
+def _draws(runner, monkeypatch):
+    """Uniform numbers by request, in the order of its steps, of a run."""
+    drawn = {}
+    plain_logits, ids = runner._logits_for, []
+
+    def logits_for(requests):
+        ids[:] = [r.request_id for r in requests]
+        return plain_logits(requests)
+
+    def sample(logits, uniforms, **kw):
+        for rid, u in zip(ids, uniforms.tolist()):
+            drawn.setdefault(rid, []).append(u)
+        return sample_tokens(logits, uniforms, **kw)
+
+    runner._logits_for = logits_for
+    with monkeypatch.context() as patch:
+        patch.setattr(llama, "sample_tokens", sample)
+        result = runner.run()
+    return drawn, result
+
+
+def test_a_request_draws_the_same_numbers_when_another_ends(monkeypatch):
+    kw = dict(temperature=1.0, seed=11, max_new_tokens=8, samples_per_prompt=2)
+    whole, result = _draws(_runner(**kw), monkeypatch)
+    assert {rid: len(v) for rid, v in whole.items()} == {rid: 8 for rid in range(6)}
+    # an end token that one request alone draws first, not at its last step
+    firsts = [tokens[:4] for tokens in result.generated_tokens]
+    eos = next(t for tokens in firsts for t in tokens if sum(t in other for other in firsts) == 1)
+    runner = _runner(**kw, eos_token_ids=[eos])
+    some, ended = _draws(runner, monkeypatch)
+    assert min(len(t) for t in ended.generated_tokens) < 8  # somebody has left early
+    for rid, numbers in some.items():
+        assert numbers == whole[rid][:len(numbers)], rid
+    assert any(len(v) == 8 for v in some.values())
