@@ -42,9 +42,9 @@ Beyond the reference's runner (all off by default):
   (128 x 128 blocks) and runs them with ``fp8_linear``;
 * ``sampler="device"`` draws a step's tokens with one ``sample_tokens`` launch
   (temperature, ``top_k``, ``top_p``, ``min_p``) from uniform numbers of one seeded
-  generator, one per request and step whoever has ended; a request whose logits leave nothing to draw (all NaN or -inf) ends with
-  the finish reason ``"error"``; ``"torch"`` is the reference's request-by-request
-  sampling;
+  generator, one per request and step whoever has ended; a request whose logits leave
+  nothing to draw (all NaN or -inf) ends with the finish reason ``"error"``;
+  ``"torch"`` is the reference's request-by-request sampling;
 * ``samples_per_prompt=n`` prefills a prompt once and forks it: the n requests share
   its full KV pages and each gets a copy of the last, partly filled one.
 
