@@ -76,9 +76,10 @@ class PrefixCache:
             found.append(block)
         return found
 
-    def match(self, tokens: Sequence[int]) -> list[int]:
-        """``lookup`` that takes the blocks: each gets one more holder (the caller
-        owns that reference and frees it like its own) and becomes most recent."""
+    def match(self, tokens: Sequence[int], owner: int | None = None) -> list[int]:
+        """``lookup`` that takes the blocks: each gets one more holder, ``owner`` if
+        given (the caller owns that reference and frees it like its own), and becomes
+        most recent."""
         usable = (len(tokens) - 1) // self.block_size
         found = []
         for key in block_keys(tokens, self.block_size, usable):
@@ -90,7 +91,7 @@ class PrefixCache:
         self.queries += usable
         self.hits += len(found)
         if found:
-            self.allocator.share(found)
+            self.allocator.share(found, owner=owner)
         return found
 
     def insert(self, tokens: Sequence[int], block_table: Sequence[int], num_tokens: int) -> int:

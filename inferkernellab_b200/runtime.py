@@ -132,7 +132,7 @@ class InferenceRuntime:
                 break
             if ids is not None:
                 del self._unplaced[request.request_id]
-                shared = self.prefix_cache.match(ids)
+                shared = self.prefix_cache.match(ids, owner=request.request_id)
                 request.cached_tokens = len(shared) * block_size
                 self.prefix_cached_tokens += request.cached_tokens
                 need = -(-max(1, request.prompt_tokens) // block_size) - len(shared)

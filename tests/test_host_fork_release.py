@@ -4,7 +4,8 @@ import itertools
 
 import pytest
 
-from inferkernellab_b200 import BlockAllocator, PagedKVCache
+from inferkernellab_b200 import (BlockAllocator, InferenceRuntime, PagedKVCache, PrefixCache,
+                                 TokenBudgetScheduler)
 
 
 @pytest.mark.parametrize("unnamed", [u for n in range(4) for u in itertools.combinations((1, 2, 3), n)])
@@ -52,3 +53,25 @@ def test_a_fork_whose_copy_fails_leaves_nothing_behind():
     # what is handed out next is what it would have been
     assert cache.allocator.allocate(6) == expected.allocator.allocate(6)
     cache.release_request(table, 1)
+
+
+@pytest.mark.parametrize("first", [1, 2, 3])
+def test_sharers_of_a_prefix_release_after_the_index_was_dropped(first):
+    """Request 2 has request 1's prompt blocks through the index, 3 is a fork of 2; the index lets
+    go of its reference while all of them still run."""
+    cache = PagedKVCache(12, 4, 2, 16, device="cpu")
+    prefix = PrefixCache(cache.allocator, 4)
+    runtime = InferenceRuntime(cache, TokenBudgetScheduler(8, 64), prefix_cache=prefix,
+                               prefill_batch_fn=lambda *a: None, decode_fn=lambda requests: None)
+    prompt = tuple(range(8))
+    requests = {1: runtime.submit(1, 8, 5, token_ids=prompt)}
+    runtime.step()
+    requests[2] = runtime.submit(2, 9, 5, token_ids=prompt + (9,))
+    runtime.step()
+    assert requests[2].block_table[:2] == requests[1].block_table[:2]
+    tables = {rid: list(r.block_table[:2]) for rid, r in requests.items()}
+    cache.allocator.share(tables[2], owner=3)
+    prefix.clear()
+    for rid in [first] + [r for r in (1, 2, 3) if r != first]:
+        cache.release_request(tables.get(rid, tables[2]), rid)
+    assert cache.allocator.num_used_blocks == 1  # request 2's own last block
