@@ -36,13 +36,17 @@
 // SMs, a cluster of CTAs splits K and joins its sums through distributed shared
 // memory in rank order (the result does not depend on timing).
 //
-// Measured on a B200, quantiser included, graph replay: 4099 tokens x 4096 x 28672 in
-// 484 us, 1990 TFLOP/s: 0.60 of twice the measured bf16 burst rate and 0.71 of twice
-// the sustained one, to which this length runs; tensor pipe active 53 % of the time.
+// Measured on a B200, quantiser included: 4099 tokens x 4096 x 28672 in 484 us in a
+// burst (graph replay), 1990 TFLOP/s, 0.60 of twice the measured bf16 burst rate; back
+// to back 554 to 566 us, 1740 to 1700 TFLOP/s, 0.61 to 0.62 of twice the sustained rate
+// (power-capped).  Tensor pipe active 53 % of the time.
 // What bounds it is the way of a block through its two accumulators: 512 clocks of
-// MMAs, the signal to the epilogue, the reads, the signal back.  64 tokens x 4096 x
-// 28672 in 28.6 us, 4.3 TB/s of weight; one token x 4096 x 6144 in 13.4 us, of which
-// the weight's bytes would take 3.9.
+// MMAs, the signal to the epilogue, the reads, the signal back, and at each block's
+// start the TMEM latency with nothing of the block before left to add.  64 tokens x 4096
+// x 28672 in 28.6 us, 4.3 TB/s of weight: 224 tiles on 296 places for CTAs, so that 76
+// SMs work on two tiles and 72 on one.  One token x 4096 x 6144 in 13.4 to 14.9 us, of
+// which the weight's bytes would take 3.9: the quantiser's launch, the pipeline's fill
+// and the join of 6 splits.
 //
 // Every mbarrier wait is bounded (1 s); on a timeout the CTA raises its abort
 // flag, records the error bit, waits (bounded) for its own copies and MMAs and

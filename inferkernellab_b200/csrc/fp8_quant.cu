@@ -5,8 +5,10 @@
 //   peak  = max |x| over the block (0 if below 2^-100)
 //   scale = peak / 448,   q = rn_e4m3(x * (448 * (1 / peak))),   x ~ q * scale
 //
-// every product and quotient rounded to 32 bits.  The peak lands on 448 (a unit in
-// the last place of 32 bits beside it at most), so nothing saturates.  A block whose
+// every product and quotient rounded to 32 bits: the order of the 32-bit torch form,
+// one rounding more than 448 / peak.  The peak lands within 2^-21 of 448 (up to a peak
+// of 2^126 within 2^-22; above it 1 / peak is subnormal), far from the next step of
+// e4m3, so nothing saturates.  A block whose
 // peak is below 2^-100 is stored as zeros with scale 0: 1 / peak would leave the
 // range of 32 bits.  A block with a NaN gets a NaN peak (the largest magnitude
 // is taken on the bit patterns, where NaN sorts above infinity), and one with

@@ -118,7 +118,9 @@ def main(argv=None) -> int:
     p.add_argument("--unfused-decode", action="store_true",
                    help="rotary append and attention as two launches per layer (A/B check)")
     p.add_argument("--projections", choices=("model", "fp8"), default="model",
-                   help="fp8: 8-bit weights and activations with block scales")
+                   help="fp8: 8-bit weights and activations with block scales (added to the "
+                        "model's 16-bit weights; faster for few requests and prefill, slower "
+                        "for large decode batches)")
     p.add_argument("--qk-norm", action="store_true",
                    help="a norm on every query and key head of every layer")
     p.add_argument("--sampler", choices=("torch", "device"), default="torch",
